@@ -261,7 +261,7 @@ def _run_plan(s):
     position = torch.where(inside, held[r] + t - start[r], 0)
     id_ = table[r, (position // page).clamp_max(width - 1)].long()
     slots = torch.where(inside & served[r] & (id_ >= 0), id_ * page + position % page, -1)
-    taken = torch.where(served, end, 0).max().clamp_min(0)
+    taken = torch.where(served & (need > 0), end, 0).max()
     tokens = stop[-1:]
     status = torch.cat([tokens, taken[None], (~served).sum()[None], (tokens - capacity).clamp_min(0)])
     return {"table": table, "seq_lens": torch.where(served, held + added, held).int(), "slots": slots,
