@@ -47,7 +47,9 @@ typedef struct ncz_driver_table {
                              const uint32_t *box, uint32_t swizzle_bytes);
     int (*set_max_dynamic_smem)(const void *kernel, int bytes);
     /* cudaLaunchKernel with a 1-D grid and block; args[i] points at the i-th
-     * kernel parameter. */
+     * kernel parameter.  Kernels that wait for the kernel before them on the
+     * device ("paged_join<..>") may be launched as its programmatic dependents,
+     * as the default table does; a plain launch is as right. */
     int (*launch_kernel)(const void *kernel, uint32_t grid, uint32_t block, size_t smem_bytes, void *stream,
                          void **args);
     int (*stream_create)(void **stream); /* non-blocking stream on the current device */
@@ -88,7 +90,7 @@ int ncz_get_driver(ncz_driver_table *out);
 
 /* Name of a kernel of the library by the host address that launch_kernel
  * receives, e.g. "flash_fwd<64,tma,f16>", "combine_splits<32>",
- * "mma_gemm<row_b>"; NCZ_ERROR_NOT_FOUND for any other address. */
+ * "mma_gemm<row_b>", "paged_decode<64,f16,1>"; NCZ_ERROR_NOT_FOUND for any other address. */
 int ncz_kernel_label(const void *kernel, char *label, size_t cap);
 
 #ifdef __cplusplus

@@ -1,6 +1,6 @@
 """Build recipe for libncz_flash.so (sm_100a only), in-tree: the flash-attention
-forward (csrc/flash_api.cu), the batched GEMM with epilogue (csrc/mma_api.cu)
-and the driver-call table both of them call CUDA through (csrc/driver.cu).
+forward (csrc/flash_api.cu), the batched GEMM with epilogue (csrc/mma_api.cu),
+the paged key-value cache (csrc/paged_api.cu) and the driver-call table all of them call CUDA through (csrc/driver.cu).
 
 libncz_flash_debug.so is the same sources with NCZ_DEBUG_ITEM_VISITS: the
 forward also counts, per work item, the CTAs that started it (a check of the
@@ -22,12 +22,12 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libncz_flash.so")
 DEBUG_LIB = os.path.join(HERE, "libncz_flash_debug.so")
 NVCC = os.environ.get("NVCC", "nvcc")
-FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
+FLAGS = ["--threads", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
          "-shared", "-I", os.path.join(ROOT, "include")]
 
 
 def sources():
-    return [os.path.join(HERE, "csrc", f) for f in ("flash_api.cu", "mma_api.cu", "driver.cu")]
+    return [os.path.join(HERE, "csrc", f) for f in ("flash_api.cu", "mma_api.cu", "paged_api.cu", "driver.cu")]
 
 
 def deps():

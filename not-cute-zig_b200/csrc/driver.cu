@@ -60,8 +60,22 @@ int rt_set_max_dynamic_smem(const void *kernel, int bytes) {
 }
 
 int rt_launch_kernel(const void *kernel, uint32_t grid, uint32_t block, size_t smem_bytes, void *stream, void **args) {
-    const cudaError_t e =
-        cudaLaunchKernel(kernel, dim3(grid), dim3(block), args, smem_bytes, static_cast<cudaStream_t>(stream));
+    cudaError_t e;
+    if (ncz::overlaps_predecessor(kernel)) {
+        cudaLaunchAttribute overlap;
+        overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        overlap.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(grid);
+        config.blockDim = dim3(block);
+        config.dynamicSmemBytes = smem_bytes;
+        config.stream = static_cast<cudaStream_t>(stream);
+        config.attrs = &overlap;
+        config.numAttrs = 1;
+        e = cudaLaunchKernelExC(&config, kernel, args);
+    } else {
+        e = cudaLaunchKernel(kernel, dim3(grid), dim3(block), args, smem_bytes, static_cast<cudaStream_t>(stream));
+    }
     // A rejected launch also sets the runtime's last error; clear it so the
     // caller's next error check sees only its own calls.
     if (e != cudaSuccess) (void)cudaGetLastError();
@@ -163,6 +177,7 @@ int ncz_set_driver(const ncz_driver_table *table, int *released) {
     if (released != nullptr) *released = st;
     ncz::reset_flash_caches();
     ncz::reset_mma_caches();
+    ncz::reset_paged_caches();
     if (table == nullptr) {
         g_active.store(&kRuntime, std::memory_order_release);
     } else {
@@ -181,6 +196,7 @@ int ncz_get_driver(ncz_driver_table *out) {
 int ncz_kernel_label(const void *kernel, char *label, size_t cap) {
     const char *name = ncz::flash_kernel_label(kernel);
     if (name == nullptr) name = ncz::mma_kernel_label(kernel);
+    if (name == nullptr) name = ncz::paged_kernel_label(kernel);
     if (name == nullptr) return NCZ_ERROR_NOT_FOUND;
     if (label != nullptr && cap > 0) {
         std::strncpy(label, name, cap - 1);

@@ -742,6 +742,8 @@ const void *combine_kernel() {
     return reinterpret_cast<const void *>(combine_splits<D>);
 }
 
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
 const char *flash_kernel_label(const void *kernel) {
     static const struct {
         const void *fn;
@@ -791,6 +793,7 @@ int ncz_shutdown(void) {
     const int released = ncz::release_flash_objects();
     ncz::reset_flash_caches();
     ncz::reset_mma_caches();
+    ncz::reset_paged_caches();
     return released;
 }
 

@@ -1,0 +1,219 @@
+"""The paged-cache C ABI on the CPU: refusals (before any launch), grids,
+kernels and workspace through the fake driver table, and the wrapper's checks."""
+import ctypes
+
+import pytest
+
+from tests import fake_driver as F
+
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
+BASE = 0x1000_0000  # fake device addresses, never dereferenced
+
+
+def status(ncz, st):
+    return ncz.flash.STATUS_NAMES[st]
+
+
+def cache(ncz, *, pages=40, page=16, kv=8, dim=64, dtype=F16, **over):
+    row = kv * dim
+    c = ncz.paged._Cache(BASE, BASE + 0x800_0000, None, None, pages, page, kv, dim, page * row, row, dim, page * row,
+                         row, dim, dtype)
+    for name, value in over.items():
+        setattr(c, name, value)
+    return c
+
+
+def decode_desc(ncz, *, batch=4, q_heads=8, dim=64, width=64, q_dtype=F16, o_dtype=F16, device=-1, ws=1 << 30, **over):
+    d = ncz.paged._Decode(BASE, BASE + 0x100_0000, None, BASE + 0x200_0000, BASE + 0x300_0000, batch, q_heads, width,
+                          width, q_heads * dim, dim, q_heads * dim, dim, 0, 0.125, q_dtype, o_dtype,
+                          BASE + 0x4000_0000, ws, device, None)
+    for name, value in over.items():
+        setattr(d, name, value)
+    return d
+
+
+def append_desc(ncz, *, tokens=10, kv=8, dim=64, dtype=F16, device=-1, **over):
+    d = ncz.paged._Append(BASE, BASE + 0x100_0000, BASE + 0x200_0000, tokens, kv * dim, dim, kv * dim, dim, dtype,
+                          device, None)
+    for name, value in over.items():
+        setattr(d, name, value)
+    return d
+
+
+def plan_desc(ncz, *, requests=10, width=32, free=100, capacity=50, page=16, device=-1, **over):
+    a = [BASE + i * 0x10_0000 for i in range(11)]
+    d = ncz.paged._Plan(*a, requests, width, width, free, capacity, page, device, None)
+    for name, value in over.items():
+        setattr(d, name, value)
+    return d
+
+
+def run(ncz, what, *structs):
+    return status(ncz, getattr(ncz.paged.lib(), what)(*(ctypes.byref(s) for s in structs)))
+
+
+def labels(ncz, launches):
+    return [ncz.driver.kernel_label(x.kernel) for x in launches]
+
+
+BAD_CACHES = [
+    ({"k": None}, "InvalidValue"), ({"v": None}, "InvalidValue"), ({"num_pages": 0}, "InvalidValue"),
+    ({"page_size": 0}, "InvalidValue"), ({"kv_heads": 0}, "InvalidValue"), ({"head_dim": 48}, "InvalidValue"),
+    ({"head_dim": 256}, "InvalidValue"), ({"dtype": F32}, "InvalidValue"), ({"dtype": 4}, "InvalidValue"),
+    ({"k_scale": BASE}, "InvalidValue"),                       # scales belong to e4m3
+    ({"k_head_stride": 32}, "InvalidValue"), ({"v_token_stride": 64}, "InvalidValue"),  # rows overlap
+    ({"k_page_stride": 0}, "InvalidValue"), ({"num_pages": 1 << 31}, "InvalidValue"),
+    ({"k_page_stride": 1 << 41}, "Overflow"), ({"k": BASE + 8}, "Misaligned"), ({"v_page_stride": 8196}, "Misaligned"),
+]
+
+
+@pytest.mark.parametrize("over,want", BAD_CACHES)
+def test_bad_caches_are_refused_by_every_call(ncz, fake, over, want):
+    c = cache(ncz, **over)
+    assert run(ncz, "ncz_paged_validate", c) == want
+    assert run(ncz, "ncz_paged_append", c, append_desc(ncz)) == want
+    assert run(ncz, "ncz_paged_decode", c, decode_desc(ncz)) == want
+    assert fake.launches == []
+
+
+def test_cache_layouts_accepted(ncz):
+    assert run(ncz, "ncz_paged_validate", cache(ncz)) == "Success"
+    # heads outermost in a page; K and V interleaved in one array of pages; padded rows
+    assert run(ncz, "ncz_paged_validate", cache(ncz, k_token_stride=64, k_head_stride=16 * 64)) == "Success"
+    assert run(ncz, "ncz_paged_validate", cache(ncz, k_page_stride=2 * 8192, v_page_stride=2 * 8192,
+                                                v=BASE + 8192 * 2)) == "Success"
+    assert run(ncz, "ncz_paged_validate", cache(ncz, k_head_stride=72, k_token_stride=576, k_page_stride=9216)) == "Success"
+    # dimensions of one element may have any stride
+    assert run(ncz, "ncz_paged_validate", cache(ncz, kv=1, k_head_stride=3, v_head_stride=0)) == "Success"
+    assert run(ncz, "ncz_paged_validate", cache(ncz, dtype=E4M3, k_scale=BASE)) == "Success"
+    assert run(ncz, "ncz_paged_validate", cache(ncz, dim=16)) == "Success"
+    assert run(ncz, "ncz_paged_validate", cache(ncz, dim=16, dtype=E4M3)) == "InvalidValue"
+
+
+@pytest.mark.parametrize("over,want", [
+    ({"q": None}, "InvalidValue"), ({"o": None}, "InvalidValue"), ({"seq_lens": None}, "InvalidValue"),
+    ({"block_table": None}, "InvalidValue"), ({"q_heads": 12}, "InvalidValue"), ({"q_heads": 0}, "InvalidValue"),
+    ({"q_dtype": BF16}, "InvalidValue"), ({"q_dtype": F32}, "InvalidValue"), ({"o_dtype": E4M3}, "InvalidValue"),
+    ({"table_stride": 63}, "InvalidValue"), ({"o_head_stride": 32}, "InvalidValue"),
+    ({"o_batch_stride": 0}, "InvalidValue"), ({"table_width": 1 << 30, "table_stride": 1 << 30}, "Overflow"),
+    ({"q": BASE + 1}, "Misaligned"), ({"o": BASE + 1}, "Misaligned"), ({"workspace": BASE + 8}, "Misaligned"),
+    ({"workspace": None}, "OutOfMemory"), ({"workspace_bytes": 1000}, "OutOfMemory"),
+    ({"q_head_stride": 1 << 41}, "Overflow"), ({"device": 64}, "InvalidDevice"),
+])
+def test_decode_refusals(ncz, fake, over, want):
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, **over)) == want
+    assert fake.launches == []
+
+
+def test_decode_accepts_transposed_and_broadcast_rows(ncz, fake):
+    # o as [q_heads][batch][dim]; one q row for every head
+    d = decode_desc(ncz, o_head_stride=4 * 64, o_batch_stride=64, q_head_stride=0)
+    assert run(ncz, "ncz_paged_decode", cache(ncz), d) == "Success"
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=0, q=None)) == "Success"
+    assert len(fake.launches) == 2
+
+
+@pytest.mark.parametrize("over,want", [
+    ({"k": None}, "InvalidValue"), ({"v": None}, "InvalidValue"), ({"slots": None}, "InvalidValue"),
+    ({"in_dtype": BF16}, "InvalidValue"), ({"in_dtype": F32}, "InvalidValue"), ({"k": BASE + 1}, "Misaligned"),
+    ({"v_token_stride": 1 << 41}, "Overflow"), ({"tokens": 1 << 31}, "InvalidValue"),
+])
+def test_append_refusals(ncz, fake, over, want):
+    assert run(ncz, "ncz_paged_append", cache(ncz), append_desc(ncz, **over)) == want
+    assert fake.launches == []
+
+
+@pytest.mark.parametrize("over,want", [
+    ({"held": None}, "InvalidValue"), ({"added": None}, "InvalidValue"), ({"seq_lens": None}, "InvalidValue"),
+    ({"block_table": None}, "InvalidValue"), ({"free_pages": None}, "InvalidValue"), ({"slots": None}, "InvalidValue"),
+    ({"free_count": None}, "InvalidValue"), ({"left": None}, "InvalidValue"), ({"page_size": 0}, "InvalidValue"),
+    ({"table_stride": 31}, "InvalidValue"), ({"slot_capacity": 1 << 31}, "InvalidValue"),
+    ({"table_width": 1 << 28, "table_stride": 1 << 28}, "Overflow"),
+])
+def test_plan_refusals(ncz, fake, over, want):
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, **over)) == want
+    assert fake.launches == []
+
+
+def test_plan_without_optional_outputs(ncz, fake):
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, positions=None, starts=None, status=None)) == "Success"
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, requests=0, held=None, added=None, seq_lens=None,
+                                                block_table=None)) == "Success"
+    assert labels(ncz, fake.launches) == ["paged_plan"] * 2
+    assert all(x.grid % 8 == 0 for x in fake.launches)  # whole clusters
+
+
+def test_decode_kernels_by_type_and_group(ncz, fake):
+    for dtype, name in ((F16, "f16"), (BF16, "bf16"), (E4M3, "e4m3")):
+        for dim in (16, 32, 64, 128):
+            if dtype == E4M3 and dim == 16:
+                continue
+            for group, rows in ((1, 1), (8, 1), (9, 2), (16, 2), (17, 4), (40, 4)):
+                fake.launches.clear()
+                d = decode_desc(ncz, q_heads=2 * group, dim=dim, q_dtype=BF16 if dtype == BF16 else F16)
+                assert run(ncz, "ncz_paged_decode", cache(ncz, kv=2, dim=dim, dtype=dtype), d) == "Success"
+                assert labels(ncz, fake.launches) == [f"paged_decode<{dim},{name},{rows}>", f"paged_join<{dim}>"]
+
+
+def test_decode_grid_and_join(ncz, fake):
+    # 64 * 16 keys at most: the grid is what is resident at once
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=100)) == "Success"
+    assert [x.grid for x in fake.launches] == [296, 296]
+    fake.launches.clear()
+    # a table of one page: one CTA per row, each whole in it, nothing to join
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=3, width=1)) == "Success"
+    assert labels(ncz, fake.launches) == ["paged_decode<64,f16,1>"] and fake.launches[0].grid == 24
+    fake.launches.clear()
+    # few rows: a join block for each row and query head
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=1, q_heads=32)) == "Success"
+    assert fake.launches[1].grid == 8 * 4
+    # a window bounds the keys too
+    fake.launches.clear()
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=1, window=100)) == "Success"
+    assert labels(ncz, fake.launches) == ["paged_decode<64,f16,1>"]
+
+
+def test_workspace_holds_every_launch(ncz, fake):
+    need = ctypes.c_size_t(0)
+    c = cache(ncz)
+    lib = ncz.paged.lib()
+    assert lib.ncz_paged_decode_workspace(ctypes.byref(c), 8, 3, ctypes.byref(need)) == 0
+    # 2 parts per CTA of 8 rows of 64 + 2 floats, and a record per CTA
+    assert need.value == 296 * 16 + (256 - 296 * 16 % 256) % 256 + 2 * 296 * 8 * 66 * 4
+    assert run(ncz, "ncz_paged_decode", c, decode_desc(ncz, ws=need.value)) == "Success"
+    assert run(ncz, "ncz_paged_decode", c, decode_desc(ncz, ws=need.value - 1)) == "OutOfMemory"
+    assert status(ncz, lib.ncz_paged_decode_workspace(ctypes.byref(c), 12, -1, ctypes.byref(need))) == "InvalidValue"
+    assert status(ncz, lib.ncz_paged_decode_workspace(ctypes.byref(c), 8, -1, None)) == "InvalidValue"
+
+
+def test_launches_go_to_the_named_device_and_count(ncz, fake):
+    before = ncz.flash.launch_count()
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, device=5)) == "Success"
+    assert run(ncz, "ncz_paged_append", cache(ncz), append_desc(ncz, device=2)) == "Success"
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, device=7)) == "Success"
+    assert [x.device for x in fake.launches] == [5, 5, 2, 7] and fake.current() == 0
+    assert ncz.flash.launch_count() - before == 4
+
+
+def test_failures_reach_the_caller(ncz, fake):
+    fake.fail("set_max_dynamic_smem", device=3, error=F.INVALID_VALUE)
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, device=3)) == "InvalidValue"
+    assert fake.launches == [] and fake.current() == 0
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, device=3)) == "Success"
+    fake.launches.clear()
+    fake.fail("launch_kernel", device=3, error=F.LAUNCH_FAILURE)
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, device=3)) == "LaunchFailed"
+    assert fake.launches == []  # no join without its decode
+    fake.fail("set_device", device=4, error=F.INVALID_DEVICE)
+    assert run(ncz, "ncz_paged_append", cache(ncz), append_desc(ncz, device=4)) == "InvalidDevice"
+    assert fake.current() == 0
+
+
+def test_wrapper_refuses_host_tensors(ncz):
+    torch = pytest.importorskip("torch")
+    pages = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    with pytest.raises(ncz.FlashError, match="CUDA"):
+        ncz.paged.Cache(pages, pages.clone())
+    ints = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ncz.FlashError, match="CUDA"):
+        ncz.paged.plan(ints, ints, ints, ints[:1], ints.view(2, 2), ints, torch.zeros(4, dtype=torch.int64), page_size=16)
