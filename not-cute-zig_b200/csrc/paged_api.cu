@@ -28,6 +28,8 @@ struct Kernel {
     const void *fn;
     const char *label;
     int smem;
+    int ctas;  // decode: CTAs per SM
+    int tile;  // decode: keys a CTA takes per step
     bool ready[kMaxDevices];
 };
 
@@ -36,12 +38,13 @@ const void *decode_fn() {
     return reinterpret_cast<const void *>(nczp::paged_decode<nczp::Decode<D, kKv, NT>>);
 }
 #define NCZ_DECODE(D, KV, KVNAME, NT) \
-    {decode_fn<D, KV, NT>(), "paged_decode<" #D "," KVNAME "," #NT ">", nczp::Decode<D, KV, NT>::kSmem, {}}
+    {decode_fn<D, KV, NT>(), "paged_decode<" #D "," KVNAME "," #NT ">", nczp::Decode<D, KV, NT>::kSmem, \
+     nczp::Decode<D, KV, NT>::kCtas, nczp::Decode<D, KV, NT>::kTile, {}}
 #define NCZ_DECODE_NT(D, KV, KVNAME) \
     {NCZ_DECODE(D, KV, KVNAME, 1), NCZ_DECODE(D, KV, KVNAME, 2), NCZ_DECODE(D, KV, KVNAME, 4)}
 #define NCZ_DECODE_D(KV, KVNAME, FIRST) \
     {FIRST, NCZ_DECODE_NT(32, KV, KVNAME), NCZ_DECODE_NT(64, KV, KVNAME), NCZ_DECODE_NT(128, KV, KVNAME)}
-#define NCZ_NONE {{nullptr, nullptr, 0, {}}, {nullptr, nullptr, 0, {}}, {nullptr, nullptr, 0, {}}}
+#define NCZ_NONE {{nullptr, nullptr, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, {}}}
 
 // [cache type - 1][log2(head_dim) - 4][log2(query heads per item / 8)]
 Kernel g_decode[3][4][3] = {
@@ -50,17 +53,17 @@ Kernel g_decode[3][4][3] = {
     NCZ_DECODE_D(nczp::kE4M3, "e4m3", NCZ_NONE),
 };
 Kernel g_join[4] = {
-    {reinterpret_cast<const void *>(nczp::paged_join<16>), "paged_join<16>", 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<32>), "paged_join<32>", 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<64>), "paged_join<64>", 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<128>), "paged_join<128>", 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<16>), "paged_join<16>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<32>), "paged_join<32>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<64>), "paged_join<64>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<128>), "paged_join<128>", 0, 0, 0, {}},
 };
 Kernel g_append[3] = {
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, false>), "paged_append<copy>", 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, true>), "paged_append<f16,e4m3>", 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kBF16, true>), "paged_append<bf16,e4m3>", 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, false>), "paged_append<copy>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, true>), "paged_append<f16,e4m3>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kBF16, true>), "paged_append<bf16,e4m3>", 0, 0, 0, {}},
 };
-Kernel g_plan = {reinterpret_cast<const void *>(nczp::paged_plan), "paged_plan", nczp::kPlanSmem, {}};
+Kernel g_plan = {reinterpret_cast<const void *>(nczp::paged_plan), "paged_plan", nczp::kPlanSmem, 0, 0, {}};
 
 template <class Fn>
 void each_kernel(Fn fn) {
@@ -181,7 +184,7 @@ Kernel &decode_kernel(const ncz_paged_cache &c, size_t group) {
 }
 
 // CTAs of a launch at most: what is resident at once.
-int max_ctas(const Kernel &k, int sms) { return sms * (k.smem > 113 * 1024 ? 1 : nczp::kCtasPerSm); }
+int max_ctas(const Kernel &k, int sms) { return sms * k.ctas; }
 
 size_t records_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(int4) + 255) / 256 * 256; }
 
@@ -195,10 +198,9 @@ int check_heads(const ncz_paged_cache &c, size_t q_heads) {
     return NCZ_SUCCESS;
 }
 
-// Keys of a step over all warps of a CTA, as nczp::Decode has it.
-int tile_keys(const ncz_paged_cache &c) {
-    const int row = static_cast<int>(c.head_dim) * element_size(c.dtype);
-    return 16 * (row >= 256 ? 1 : row >= 64 ? 2 : 4) * nczp::kWarps;
+// Whether a launch's CTAs each stay with one head block (nczp::paged_decode's by_head).
+bool choose_by_head(size_t head_blocks, size_t ctas) {
+    return head_blocks > 1 && head_blocks <= ctas && (ctas % head_blocks) * 16 <= ctas;
 }
 
 }  // namespace
@@ -368,7 +370,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     p.num_pages = static_cast<int>(c.num_pages);
     p.page = fast_div(static_cast<uint32_t>(c.page_size));
     p.scale_log2 = static_cast<float>(static_cast<double>(d.scale) * 1.4426950408889634);
-    p.min_tiles = 1;
+    p.whole_groups = c.page_size % 16 == 0;
     p.q_bf16 = d.q_dtype == NCZ_DTYPE_BF16;
     p.o_dtype = d.o_dtype;
     p.q_vec = aligned(d.q, 8) && d.q_batch_stride % 4 == 0 && d.q_head_stride % 4 == 0;
@@ -382,11 +384,14 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         if (!aligned(d.workspace, 16)) return static_cast<int>(NCZ_ERROR_MISALIGNED);
         // Tiles at most: the lengths are on the device, the table's width bounds them.
         const size_t keys = d.window > 0 ? std::min(d.window, static_cast<size_t>(p.width_keys)) : p.width_keys;
-        const size_t most = std::max<size_t>(1, (keys + tile_keys(c) - 1) / tile_keys(c));
+        const size_t tile = static_cast<size_t>(k.tile);
+        const size_t most = std::max<size_t>(1, (keys + (d.window > 0 ? 15 : 0) + tile - 1) / tile);
         const size_t items = d.batch * static_cast<size_t>(p.head_blocks);
         const int ctas = max_ctas(k, sms);
-        const unsigned grid = static_cast<unsigned>(
+        unsigned grid = static_cast<unsigned>(
             most > static_cast<size_t>(ctas) ? ctas : std::min(static_cast<size_t>(ctas), most * items));
+        p.by_head = choose_by_head(static_cast<size_t>(p.head_blocks), grid);
+        if (p.by_head) grid -= grid % static_cast<unsigned>(p.head_blocks);
         p.records_by_item = items <= grid;
         char *ws = static_cast<char *>(d.workspace);
         p.records = reinterpret_cast<int4 *>(ws);

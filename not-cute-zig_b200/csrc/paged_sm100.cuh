@@ -332,58 +332,53 @@ struct DecodeParams {
     long long k_page, k_tok, k_head, v_page, v_tok, v_head;  // bytes
     long long q_batch, q_head, o_batch, o_head, table_stride;  // elements
     int batch, group, blocks, head_blocks;  // query heads per K/V head; blocks of them; kv_heads * blocks
-    int width_keys, window, num_pages, page_size;
+    int width_keys, window, num_pages;
+    int whole_groups;  // page_size is a multiple of 16: the 16 keys of a group lie in one page
+    int by_head;       // every CTA stays with one head block (see paged_decode)
     FastDiv page;
     float scale_log2;
-    int min_tiles, records_by_item;
+    int records_by_item;
     int q_bf16, o_dtype, q_vec, o_vec, p_parts;
 };
 
 constexpr int kWarps = 4;
 constexpr int kDecodeThreads = kWarps * 32;
-constexpr int kCtasPerSm = 2;
-constexpr int kMaxKeys = 0x7FFFFFFF;
 
-// Copies of one 16-key group: a lane takes kKChunk bytes of the K rows g and
-// g + 8 (g = lane / 4; four lanes side by side cover a row) and kVChunk bytes
-// of the V rows 2t, 2t + 1, 2t + 8, 2t + 9 (t = lane % 4; eight lanes cover a
-// row).  Those are exactly the rows of that lane's matrix fragments, so a
-// lane reads back only bytes it copied itself and the ring needs no barrier.
-template <int D_, int kKv_, int NT_>
+// One instantiation: head_dim, cache type, and the query heads of an item, 8
+// (one matrix column block, NT = 1), 16 (NT = 2) or 32 (NT = 2, two warps
+// sharing each slice of keys, kShare = 2).
+template <int D_, int kKv_, int kBlocks_>
 struct Decode {
-    static constexpr int D = D_, kKv = kKv_, NT = NT_;
+    static constexpr int D = D_, kKv = kKv_;
+    static constexpr int NT = kBlocks_ > 1 ? 2 : 1;
+    static constexpr int kShare = kBlocks_ / NT;
+    static constexpr int kRows = 8 * kBlocks_;
     static constexpr int kEl = kKv == kE4M3 ? 1 : 2;
-    static constexpr int kRow = D * kEl;
-    static constexpr int kKChunk = kRow / 4 < 16 ? kRow / 4 : 16;
-    static constexpr int kKChunks = kRow / (4 * kKChunk);
-    static constexpr int kVChunk = kRow / 8 < 16 ? kRow / 8 : 16;
-    static constexpr int kVChunks = kRow / (8 * kVChunk);
-    static constexpr int KS = kRow >= 256 ? 1 : (kRow >= 64 ? 2 : 4);  // 16-key groups per step
-    static constexpr int kKeys = 16 * KS;                              // keys per warp and step
-    static constexpr int kTile = kKeys * kWarps;                       // keys per CTA and step
-    static constexpr int kStage = kKeys * kRow * 2;                    // bytes per warp
-    static constexpr int kStages = 24576 / kStage < 6 ? 24576 / kStage : 6;
-    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kRow = D * kEl;              // bytes of a row of K or V
+    static constexpr int kChunks = kRow / 16;         // 16-byte chunks of a row
+    static constexpr int kRowsPerCopy = 32 / kChunks; // rows a warp's copy instruction covers
+    static constexpr int kCopies = 16 / kRowsPerCopy; // copy instructions of 16 rows
+    static constexpr int KS = kShare * (kRow >= 256 ? 1 : kRow >= 64 ? 2 : 4);  // 16-key groups per step
+    static constexpr int kKeys = 16 * KS;                                       // keys per slice and step
+    static constexpr int kSlices = kWarps / kShare;
+    static constexpr int kTile = kKeys * kSlices;      // keys per CTA and step
+    static constexpr int kStage = kKeys * kRow * 2;    // bytes per slice
+    static constexpr int kCtas = NT == 1 ? 3 : 2;      // CTAs per SM
+    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024) / kSlices / kStage;
+    static constexpr int kStages = kFit < 6 ? kFit : 6;
+    static constexpr int kSmem = kSlices * kStages * kStage;
     static constexpr int kMaskWords = (kKeys + 31) / 32;
-    static constexpr int kRows = 8 * NT;    // query heads of an item
-    static constexpr int kCombStride = D + 4;
-    static constexpr bool kQSmem = D * NT > 256;  // Q fragments in shared memory where registers do not hold them
-    static constexpr int kQBytes = kQSmem ? (D / 16) * NT * 32 * 8 : 0;
-    static constexpr int kComb = kWarps * 8 * kCombStride * 4;
-    static constexpr int kSmem = kRing + kComb + kQBytes;
-    static constexpr int MT = D / 16;       // 16-row blocks of O^T
-    static constexpr int CE = kKChunk / kEl, VE = kVChunk / kEl;
+    static constexpr int kCombStride = D + 4;          // floats; 4 apart: no bank conflicts when warps write
+    static constexpr int MT = D / 16;                  // 16-row blocks of O^T
+    static_assert(kStages >= 2 && kShare * 8 * kCombStride * 4 <= kStage, "");
 };
 
-template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const char *src, uint32_t bytes) {
-    if constexpr (kBytes == 16) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-    } else if constexpr (kBytes == 8) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-    } else {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-    }
+__device__ __forceinline__ void copy16(uint32_t dst, const char *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 16 bytes, or zeros where bytes is 0 (src is not read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const char *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n>
@@ -391,31 +386,33 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
 }
 
-template <int kBytes>
-__device__ __forceinline__ void load_chunk(uint32_t (&r)[kBytes / 4], uint32_t addr) {
-    if constexpr (kBytes == 16) {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-    } else if constexpr (kBytes == 8) {
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
-    } else {
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
-    }
+// Swizzle of a tile of rows of kRow bytes: the 16-byte chunk at which chunk 0
+// of a row starts (xor), such that 8 rows' equal chunks lie in different banks.
+template <int kRow>
+__device__ __forceinline__ uint32_t chunk_xor(uint32_t row) {
+    return kRow >= 128 ? row & 7 : kRow == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
 template <bool kBf16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
     if constexpr (kBf16) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     } else {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
 }
 
@@ -425,7 +422,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return r;
 }
 
-// Two f16 of the e4m3 pair in the low or high half of w (exact).
+// Two f16 of the e4m3 pair in the low half of w (exact).
 __device__ __forceinline__ uint32_t e4m3_f16x2(uint32_t pair) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(pair)));
@@ -437,25 +434,28 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return kBf16 ? ncz::pack_bf16x2(lo, hi) : ncz::pack_f16x2(lo, hi);
 }
 
-// Keys of request b: [lo, hi), in `tiles` tiles (one at least, so that every
-// request's rows are written).
+// Keys of request b: [lo, hi), in `tiles` tiles from lo rounded down to 16
+// (one tile at least, so that every request's rows are written).
 template <int kTile>
 __device__ __forceinline__ void request_keys(const DecodeParams &p, int b, int &lo, int &hi, int &tiles) {
     hi = min(max(__ldg(p.lens + b), 0), p.width_keys);
     lo = p.window > 0 ? max(0, hi - p.window) : 0;
-    tiles = max(1, (hi - lo) / kTile + ((hi - lo) % kTile != 0));
+    const uint32_t n = static_cast<uint32_t>(hi - (lo & ~15));
+    tiles = max(1, static_cast<int>(n / kTile + (n % kTile != 0)));
 }
 
-// Where a CTA stands in the launch's list of tiles: request-major, then K/V
-// head, then block of query heads, then tile.
+// Where a CTA stands in its list of tiles: request-major, then head block
+// (unless the CTA stays with one), then tile.
 template <int kTile>
 struct Cursor {
     int b, hb, tile, tiles, lo, hi;
     __device__ __forceinline__ void advance(const DecodeParams &p) {
         if (++tile < tiles) return;
         tile = 0;
-        if (++hb < p.head_blocks) return;
-        hb = 0;
+        if (!p.by_head) {
+            if (++hb < p.head_blocks) return;
+            hb = 0;
+        }
         if (++b < p.batch) request_keys<kTile>(p, b, lo, hi, tiles);
     }
 };
@@ -494,31 +494,43 @@ __device__ __forceinline__ void finish_quad(const DecodeParams &p, int b, int kv
 
 // The base of the exponentials is kept kLift below the largest score seen
 // when it was set, and raised only when a score passes it by kTop: P then
-// lies in (0, 2^kTop], under the largest f16 value, keys 2^-kLift of the
-// f16 range's bottom above what a base at the maximum would keep, and O is
+// lies in (0, 2^kTop], under the largest f16 value, and keys 2^-kLift further
+// down than with a base at the maximum stay above the smallest f16.  O is
 // rescaled rarely (on the first keys, and where scores grow by 2^(kTop-kLift)).
 constexpr float kLift = 8.0f, kTop = 15.0f;
 
 template <class T>
-__global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kCtasPerSm)
-    paged_decode(const DecodeParams p) {
+__global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const DecodeParams p) {
     constexpr int D = T::D, NT = T::NT, KS = T::KS, MT = T::MT, S = T::kStages;
     constexpr bool kBf16 = T::kKv == kBF16, k8 = T::kKv == kE4M3;
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(128) char smem[];
     __shared__ long long warp_sums[kWarps];
     __shared__ int s_start[3];
     __shared__ uint32_t s_mask[kWarps][S][T::kMaskWords];
     __shared__ float s_ml[kWarps][8][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
-    float *const comb = reinterpret_cast<float *>(smem + T::kRing);
-    const uint32_t ring = smem_u32(smem) + warp * (S * T::kStage);
+    const int slice = warp / T::kShare, part = warp % T::kShare;  // slice of keys, part of the query heads
+    const uint32_t ring = smem_u32(smem) + slice * (S * T::kStage);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+    // The warps that share a slice of keys: wait for each other's copies and reads.
+    auto slice_sync = [&]() {
+        if constexpr (T::kShare == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + slice), "n"(T::kShare * 32) : "memory");
+    };
+
     // This CTA's share of the launch's tiles: each CTA sums the requests' tile
-    // counts itself (a few KB of lengths), then takes an equal run of tiles.
-    long long first, last;  // [first, last)
-    long long per;
+    // counts itself (a few KB of lengths), then takes an equal run of them.
+    // by_head: CTA c works on head block c % head_blocks alone, on the run
+    // c / head_blocks of the tiles of all requests, so that the CTAs that read
+    // one page's heads do so at the same time.
+    const int unit_heads = p.by_head ? 1 : p.head_blocks;
+    const int runs = p.by_head ? gridDim.x / p.head_blocks : gridDim.x;
+    const int run = p.by_head ? blockIdx.x / p.head_blocks : blockIdx.x;
+    long long first, last, per;
     Cursor<T::kTile> at;
     {
         const int chunk = (p.batch + kDecodeThreads - 1) / kDecodeThreads;
@@ -527,7 +539,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
         for (int b = b0; b < b1; ++b) {
             int lo, hi, tiles;
             request_keys<T::kTile>(p, b, lo, hi, tiles);
-            mine += static_cast<long long>(tiles) * p.head_blocks;
+            mine += static_cast<long long>(tiles) * unit_heads;
         }
         long long upto = mine;  // inclusive prefix over the warp, then exclusive over the block
 #pragma unroll
@@ -543,8 +555,8 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
             if (w < warp) before += warp_sums[w];
             total += warp_sums[w];
         }
-        per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_tiles));
-        first = blockIdx.x * per;
+        per = (total + runs - 1) / runs;
+        first = run * per;
         last = min(first + per, total);
         if (first >= last) {
             if (tid == 0 && !p.records_by_item) p.records[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -555,7 +567,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
             for (int b = b0; b < b1; ++b) {
                 int lo, hi, tiles;
                 request_keys<T::kTile>(p, b, lo, hi, tiles);
-                const long long n = static_cast<long long>(tiles) * p.head_blocks;
+                const long long n = static_cast<long long>(tiles) * unit_heads;
                 if (first < x + n) {
                     s_start[0] = b;
                     s_start[1] = static_cast<int>((first - x) / tiles);
@@ -567,72 +579,111 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
         }
         __syncthreads();
         at.b = s_start[0];
-        at.hb = s_start[1];
+        at.hb = p.by_head ? static_cast<int>(blockIdx.x % p.head_blocks) : s_start[1];
         at.tile = s_start[2];
         request_keys<T::kTile>(p, at.b, at.lo, at.hi, at.tiles);
     }
 
     // ---- producer side: the step being prepared is `ahead`; its keys' page
-    // ids are loaded one step before its rows are copied.
-    constexpr int kOwn = T::kMaskWords;  // keys a lane looks up per step
+    // ids are loaded one step before its rows are copied.  A copy instruction
+    // moves whole rows (kRowsPerCopy of them): lane / kChunks is its row,
+    // lane % kChunks its 16-byte chunk.
+    constexpr int kIds = KS > T::kMaskWords ? KS : T::kMaskWords;
     Cursor<T::kTile> ahead = at;
     long long ahead_left = last - first;
-    int ids[kOwn];
+    int ids[kIds];
+    const int row = lane / T::kChunks, chunk = lane % T::kChunks;
+    const long long k_lane = row * p.k_tok + chunk * 16, v_lane = row * p.v_tok + chunk * 16;
+    auto first_key = [&](const Cursor<T::kTile> &c) {  // of this warp's slice, a multiple of 16
+        return static_cast<uint32_t>(c.lo & ~15) + static_cast<uint32_t>(c.tile) * T::kTile + slice * T::kKeys;
+    };
     auto look_up = [&]() {
+        if (ahead_left <= 0) return;
+        const int *const table = p.table + ahead.b * p.table_stride;
+        const uint32_t key0 = first_key(ahead), hi = ahead.hi;
+        if (p.whole_groups) {
+            // One id per group of 16 keys, the same in every lane.
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const long long key = static_cast<long long>(ahead.lo) + static_cast<long long>(ahead.tile) * T::kTile +
-                                  warp * T::kKeys + i * 32 + lane;
-            ids[i] = -1;
-            if (ahead_left > 0 && i * 32 + lane < T::kKeys && key < ahead.hi)
-                ids[i] = __ldg(p.table + ahead.b * p.table_stride + p.page.div(static_cast<uint32_t>(key)));
+            for (int i = 0; i < KS; ++i)
+                ids[i] = key0 + i * 16 < hi ? __ldg(table + p.page.div(key0 + i * 16)) : -1;
+        } else {
+            // Key i * 32 + lane's id.
+#pragma unroll
+            for (int i = 0; i < T::kMaskWords; ++i) {
+                const uint32_t key = key0 + i * 32 + lane;
+                ids[i] = i * 32 + lane < T::kKeys && key < hi ? __ldg(table + p.page.div(key)) : -1;
+            }
         }
     };
     auto produce = [&](int stage) {
         if (ahead_left > 0) {
             const int kv_head = p.blocks == 1 ? ahead.hb : ahead.hb / p.blocks;
             const char *const kb = p.k + kv_head * p.k_head, *const vb = p.v + kv_head * p.v_head;
-            long long k_off[kOwn], v_off[kOwn];
-            uint32_t any = 0;
+            const uint32_t key0 = first_key(ahead), lo = ahead.lo, hi = ahead.hi;
+            const uint32_t k_dst = ring + stage * T::kStage, v_dst = k_dst + T::kKeys * T::kRow;
+            uint32_t mask[T::kMaskWords];
+            if (p.whole_groups) {
 #pragma unroll
-            for (int i = 0; i < kOwn; ++i) {
-                const uint32_t key = static_cast<uint32_t>(ahead.lo) + static_cast<uint32_t>(ahead.tile) * T::kTile +
-                                     warp * T::kKeys + i * 32 + lane;  // used only where it is below hi
-                const bool ok = ids[i] >= 0 && ids[i] < p.num_pages;
-                const int row = ok ? static_cast<int>(key - p.page.div(key) * p.page.d) : 0;
-                k_off[i] = ok ? ids[i] * p.k_page + row * p.k_tok : -1;
-                v_off[i] = ok ? ids[i] * p.v_page + row * p.v_tok : -1;
-                const uint32_t mask = __ballot_sync(~0u, ok);
-                any |= mask;
-                if (lane == 0) s_mask[warp][stage][i] = mask;
-            }
-            if (any != 0) {
-                const uint32_t k_dst = ring + stage * T::kStage + lane * T::kKChunk;
-                const uint32_t v_dst = ring + stage * T::kStage + T::kKeys * T::kRow + lane * T::kVChunk;
+                for (int i = 0; i < T::kMaskWords; ++i) mask[i] = 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t key = key0 + ks * 16;
+                    if (static_cast<uint32_t>(ids[ks]) < static_cast<uint32_t>(p.num_pages)) {  // hence key < hi
+                        uint32_t m = hi - key < 16 ? (1u << (hi - key)) - 1 : 0xFFFFu;
+                        if (key < lo) m &= lo - key < 16 ? ~((1u << (lo - key)) - 1) : 0u;
+                        mask[ks / 2] |= m << (ks % 2 * 16);
+                        const uint32_t in_page = key - p.page.div(key) * p.page.d;
+                        const char *k_src = kb + (ids[ks] * p.k_page + in_page * p.k_tok) + k_lane;
+                        const char *v_src = vb + (ids[ks] * p.v_page + in_page * p.v_tok) + v_lane;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const long long off = __shfl_sync(~0u, k_off[ks / 2], (ks * 16 + r * 8 + g) & 31);
-                        const char *src = kb + (off >= 0 ? off + t4 * T::kKChunk : 0);
-                        const uint32_t bytes = off >= 0 ? T::kKChunk : 0;
-#pragma unroll
-                        for (int c = 0; c < T::kKChunks; ++c)
-                            copy_async<T::kKChunk>(k_dst + ((ks * 2 + r) * T::kKChunks + c) * (32 * T::kKChunk),
-                                                   src + (off >= 0 ? c * 4 * T::kKChunk : 0), bytes);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const long long off =
-                            __shfl_sync(~0u, v_off[ks / 2], (ks * 16 + (r >> 1) * 8 + t4 * 2 + (r & 1)) & 31);
-                        const char *src = vb + (off >= 0 ? off + g * T::kVChunk : 0);
-                        const uint32_t bytes = off >= 0 ? T::kVChunk : 0;
-#pragma unroll
-                        for (int c = 0; c < T::kVChunks; ++c)
-                            copy_async<T::kVChunk>(v_dst + ((ks * 4 + r) * T::kVChunks + c) * (32 * T::kVChunk),
-                                                   src + (off >= 0 ? c * 8 * T::kVChunk : 0), bytes);
+                        for (int j = 0; j < T::kCopies; ++j) {
+                            const uint32_t r = ks * 16 + j * T::kRowsPerCopy + row;
+                            const uint32_t to = r * T::kRow + ((chunk ^ chunk_xor<T::kRow>(r)) << 4);
+                            if ((ks * T::kCopies + j) % T::kShare == part) {
+                                if (m == 0xFFFFu) {
+                                    copy16(k_dst + to, k_src);
+                                    copy16(v_dst + to, v_src);
+                                } else {
+                                    const uint32_t bytes = ((m >> (r & 15)) & 1) * 16;
+                                    copy16(k_dst + to, k_src, bytes);
+                                    copy16(v_dst + to, v_src, bytes);
+                                }
+                            }
+                            k_src += T::kRowsPerCopy * p.k_tok;
+                            v_src += T::kRowsPerCopy * p.v_tok;
+                        }
                     }
                 }
+            } else {
+                long long k_off[T::kMaskWords], v_off[T::kMaskWords];
+#pragma unroll
+                for (int i = 0; i < T::kMaskWords; ++i) {
+                    const uint32_t key = key0 + i * 32 + lane;
+                    const bool ok = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(p.num_pages) && key >= lo;
+                    const uint32_t in_page = ok ? key - p.page.div(key) * p.page.d : 0;
+                    k_off[i] = ok ? ids[i] * p.k_page + in_page * p.k_tok : -1;
+                    v_off[i] = ok ? ids[i] * p.v_page + in_page * p.v_tok : -1;
+                    mask[i] = __ballot_sync(~0u, ok);
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (((mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu) == 0) continue;
+#pragma unroll
+                    for (int j = 0; j < T::kCopies; ++j) {
+                        if ((ks * T::kCopies + j) % T::kShare != part) continue;
+                        const uint32_t r = ks * 16 + j * T::kRowsPerCopy + row;
+                        const uint32_t to = r * T::kRow + ((chunk ^ chunk_xor<T::kRow>(r)) << 4);
+                        const long long ko = __shfl_sync(~0u, k_off[ks / 2], r & 31);
+                        const long long vo = __shfl_sync(~0u, v_off[ks / 2], r & 31);
+                        const uint32_t bytes = ko >= 0 ? 16 : 0;
+                        copy16(k_dst + to, kb + (ko >= 0 ? ko + chunk * 16 : 0), bytes);
+                        copy16(v_dst + to, vb + (vo >= 0 ? vo + chunk * 16 : 0), bytes);
+                    }
+                }
+            }
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < T::kMaskWords; ++i) s_mask[warp][stage][i] = mask[i];
             }
             ahead.advance(p);
             --ahead_left;
@@ -645,45 +696,51 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) produce(s);
 
-    // ---- consumer side
+    // ---- consumer side.  Scores S^T = K Q^T (keys as rows), O^T = V^T P^T (head_dim as rows).
     float acc[MT][NT][4];  // O^T: rows g and g + 8 of block mt, query heads 2 t4 and 2 t4 + 1
     float base[NT][2], sum[NT][2];
-    uint32_t qf[T::kQSmem ? 1 : D / 16][NT][2];
+    uint32_t qf[D / 16][NT][2];
     float q_up[NT][2];  // power of two taken out of a query head's elements (bf16 q against an e4m3 cache)
-    uint2 *const s_q = reinterpret_cast<uint2 *>(smem + T::kRing + T::kComb);
     bool fresh = true;
     bool head_cut = at.tile != 0;  // this CTA's first item began in another CTA
     int stage = 0;
     float scale = 0.0f;
+    // Rows and chunks of this lane's ldmatrix addresses: matrices 0..3 of K are
+    // (keys 0-7 | 8-15) x (chunk, chunk + 1); those of V (trans) the same for e4m3 and
+    // (chunk, chunk + 1) x (keys 0-7 | 8-15) for 16-bit types.
+    const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk = lane >> 4;
+    const uint32_t v_row = k8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_chunk = k8 ? k_chunk : (lane >> 3) & 1;
+    const uint32_t k_at = k_row * T::kRow, k_xor = chunk_xor<T::kRow>(k_row);
+    const uint32_t v_at = v_row * T::kRow, v_xor = chunk_xor<T::kRow>(v_row);
+
     for (long long step = first; step < last; ++step) {
         if (fresh) {
             fresh = false;
             const int kv_head = p.blocks == 1 ? at.hb : at.hb / p.blocks;
-            const int head0 = (at.hb - kv_head * p.blocks) * T::kRows;  // first query head of the group
+            const int head0 = (at.hb - kv_head * p.blocks) * T::kRows + part * (8 * NT);  // of the group
             scale = p.scale_log2 * (k8 && p.k_scale != nullptr ? __ldg(p.k_scale + kv_head) : 1.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int head = head0 + nt * 8 + g;
                 const uint16_t *q = reinterpret_cast<const uint16_t *>(p.q) + at.b * p.q_batch +
                                     (static_cast<long long>(kv_head) * p.group + head) * p.q_head;
-                uint32_t w[D / 16][2];
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    // The elements of this lane's pieces of the K rows, in their order.
-                    const int d = (kk / (T::CE / 4)) * (4 * T::CE) + t4 * T::CE + (kk % (T::CE / 4)) * 4;
-                    if (head >= p.group) {
-                        w[kk][0] = w[kk][1] = 0;
-                    } else if (p.q_vec) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q + d));
-                        w[kk][0] = x.x;
-                        w[kk][1] = x.y;
-                    } else {
-                        w[kk][0] = q[d] | (static_cast<uint32_t>(q[d + 1]) << 16);
-                        w[kk][1] = q[d + 2] | (static_cast<uint32_t>(q[d + 3]) << 16);
+                    // The elements that meet this lane's columns of the K fragments.
+                    uint32_t(&w)[2] = qf[kk][nt];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = kk * 16 + (k8 ? 4 * t4 + 2 * j : 2 * t4 + 8 * j);
+                        if (head >= p.group)
+                            w[j] = 0;
+                        else if (p.q_vec)
+                            w[j] = __ldg(reinterpret_cast<const uint32_t *>(q + d));
+                        else
+                            w[j] = q[d] | (static_cast<uint32_t>(q[d + 1]) << 16);
                     }
                 }
-                float up = 1.0f;
                 if constexpr (k8) {
+                    float up = 1.0f;
                     if (p.q_bf16) {
                         // bf16 spans more than f16: take a power of two out of the row, so
                         // that its largest element lies in [1, 2); what f16 then rounds is below
@@ -693,7 +750,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float2 f = unpack16<true>(w[kk][j]);
+                                const float2 f = unpack16<true>(qf[kk][nt][j]);
                                 top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                             }
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -707,22 +764,12 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float2 f = unpack16<true>(w[kk][j]);
-                                w[kk][j] = ncz::pack_f16x2(f.x * down, f.y * down);
+                                const float2 f = unpack16<true>(qf[kk][nt][j]);
+                                qf[kk][nt][j] = ncz::pack_f16x2(f.x * down, f.y * down);
                             }
                     }
                     q_up[nt][0] = __shfl_sync(~0u, up, (2 * t4) * 4);
                     q_up[nt][1] = __shfl_sync(~0u, up, (2 * t4 + 1) * 4);
-                }
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    if constexpr (T::kQSmem) {
-                        // All warps hold the same fragments: each writes the same bytes.
-                        s_q[(kk * NT + nt) * 32 + lane] = make_uint2(w[kk][0], w[kk][1]);
-                    } else {
-                        qf[kk][nt][0] = w[kk][0];
-                        qf[kk][nt][1] = w[kk][1];
-                    }
                 }
                 base[nt][0] = base[nt][1] = -INFINITY;
                 sum[nt][0] = sum[nt][1] = 0.0f;
@@ -731,19 +778,18 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[mt][nt][e] = 0.0f;
             }
-            if constexpr (T::kQSmem) __syncwarp();
         }
 
         copy_wait<S - 2>();
-        __syncwarp();  // lane 0's mask words of this stage; every lane is done with the stage before it
+        slice_sync();  // this stage's rows and mask are there; every lane is done with the stage before it
         produce(stage == 0 ? S - 1 : stage - 1);
         uint32_t mask[T::kMaskWords];
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < T::kMaskWords; ++i) any |= mask[i] = s_mask[warp][stage][i];
         if (any != 0) {
-            const uint32_t k_src = ring + stage * T::kStage + lane * T::kKChunk;
-            const uint32_t v_src = ring + stage * T::kStage + T::kKeys * T::kRow + lane * T::kVChunk;
+            const uint32_t k_src = ring + stage * T::kStage + k_at;
+            const uint32_t v_src = ring + stage * T::kStage + T::kKeys * T::kRow + v_at;
             float s[KS][NT][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -752,42 +798,27 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[ks][nt][e] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < T::kKChunks; ++c) {
-                    uint32_t ra[T::kKChunk / 4], rb[T::kKChunk / 4];
-                    load_chunk<T::kKChunk>(ra, k_src + ((ks * 2 + 0) * T::kKChunks + c) * (32 * T::kKChunk));
-                    load_chunk<T::kKChunk>(rb, k_src + ((ks * 2 + 1) * T::kKChunks + c) * (32 * T::kKChunk));
-#pragma unroll
-                    for (int i = 0; i < T::CE / 4; ++i) {
-                        uint32_t a0, a1, a2, a3;
-                        if constexpr (k8) {
-                            a0 = e4m3_f16x2(ra[i]);
-                            a1 = e4m3_f16x2(rb[i]);
-                            a2 = e4m3_f16x2(ra[i] >> 16);
-                            a3 = e4m3_f16x2(rb[i] >> 16);
-                        } else {
-                            a0 = ra[2 * i];
-                            a1 = rb[2 * i];
-                            a2 = ra[2 * i + 1];
-                            a3 = rb[2 * i + 1];
-                        }
-                        const int kk = c * (T::CE / 4) + i;
+                for (int c = 0; c < T::kChunks; c += 2) {
+                    uint32_t r[4];
+                    ldmatrix4(r, k_src + ks * 16 * T::kRow + (((k_chunk + c) ^ k_xor) << 4));
+                    if constexpr (k8) {
+                        // A chunk is 16 elements: two products.
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            uint32_t b0, b1;
-                            if constexpr (T::kQSmem) {
-                                const uint2 x = s_q[(kk * NT + nt) * 32 + lane];
-                                b0 = x.x;
-                                b1 = x.y;
-                            } else {
-                                b0 = qf[kk][nt][0];
-                                b1 = qf[kk][nt][1];
-                            }
-                            mma16816<kBf16>(s[ks][nt], a0, a1, a2, a3, b0, b1);
+                            mma16816<false>(s[ks][nt], e4m3_f16x2(r[0]), e4m3_f16x2(r[1]), e4m3_f16x2(r[0] >> 16),
+                                            e4m3_f16x2(r[1] >> 16), qf[c][nt][0], qf[c][nt][1]);
+                            mma16816<false>(s[ks][nt], e4m3_f16x2(r[2]), e4m3_f16x2(r[3]), e4m3_f16x2(r[2] >> 16),
+                                            e4m3_f16x2(r[3] >> 16), qf[c + 1][nt][0], qf[c + 1][nt][1]);
                         }
+                    } else {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816<kBf16>(s[ks][nt], r[0], r[1], r[2], r[3], qf[c / 2][nt][0], qf[c / 2][nt][1]);
                     }
                 }
             }
-            // Scores in log2 units; keys outside the mask -infinity.
+            // Scores in log2 units; keys outside the mask -infinity (their rows may be
+            // zeros or, where a whole group is absent, an older step's).
             bool grow = false;
             float top[NT][2];
 #pragma unroll
@@ -828,7 +859,6 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                         }
                     }
             }
-            uint32_t pb[KS][NT][2][2];  // [part][key half]: P^T fragments
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float m0 = base[nt][0] == -INFINITY ? 0.0f : base[nt][0];
@@ -844,7 +874,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                     sum[nt][1] += x[1] + x[3];
                 }
             }
-            // P in 16-bit parts: each takes the rounded value and leaves the rest to the next.
+            // P^T fragments in 16-bit parts: each takes the rounded value and leaves the rest to the next.
             auto next_part = [&](int ks, int nt, uint32_t (&b)[2]) {
                 float(&x)[4] = s[ks][nt];
 #pragma unroll
@@ -857,71 +887,64 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                 }
             };
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (KS > 1)
+                    if (((mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu) == 0) continue;  // V's rows are not there
+                uint32_t b[3][NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    next_part(ks, nt, pb[ks][nt][0]);
-                    next_part(ks, nt, pb[ks][nt][1]);
-                }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t third[NT][2];
-                if constexpr (kBf16) {
-                    if (p.p_parts > 2) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) next_part(ks, nt, third[nt]);
+                    next_part(ks, nt, b[0][nt]);
+                    next_part(ks, nt, b[1][nt]);
+                    if constexpr (kBf16) {
+                        if (p.p_parts > 2) next_part(ks, nt, b[2][nt]);
                     }
                 }
+                // The products of one group are summed apart and then added: the matrix unit's own
+                // additions cut off below 2^-24 of the sum, always downwards in magnitude.
+                auto block = [&](int mt, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                for (int c = 0; c < T::kVChunks; ++c) {
-                    uint32_t r[4][T::kVChunk / 4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        load_chunk<T::kVChunk>(r[i], v_src + ((ks * 4 + i) * T::kVChunks + c) * (32 * T::kVChunk));
-#pragma unroll
-                    for (int m = 0; m < T::VE / 2; ++m) {
-                        // Rows of V^T: two elements of each row, keys paired.
-                        uint32_t a0, a1, a2, a3;
-                        if constexpr (k8) {
-                            const uint32_t sel = m % 2 == 0 ? 0x5140 : 0x7362;
-                            const uint32_t x = __byte_perm(r[0][m / 2], r[1][m / 2], sel);
-                            const uint32_t y = __byte_perm(r[2][m / 2], r[3][m / 2], sel);
-                            a0 = e4m3_f16x2(x);
-                            a1 = e4m3_f16x2(x >> 16);
-                            a2 = e4m3_f16x2(y);
-                            a3 = e4m3_f16x2(y >> 16);
-                        } else {
-                            a0 = __byte_perm(r[0][m], r[1][m], 0x5410);
-                            a1 = __byte_perm(r[0][m], r[1][m], 0x7632);
-                            a2 = __byte_perm(r[2][m], r[3][m], 0x5410);
-                            a3 = __byte_perm(r[2][m], r[3][m], 0x7632);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (kBf16) {
+                            if (p.p_parts > 2) mma16816<kBf16>(x, a0, a1, a2, a3, b[2][nt][0], b[2][nt][1]);
                         }
-                        const int mt = c * (T::VE / 2) + m;
+                        mma16816<kBf16>(x, a0, a1, a2, a3, b[1][nt][0], b[1][nt][1]);
+                        mma16816<kBf16>(x, a0, a1, a2, a3, b[0][nt][0], b[0][nt][1]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma16816<kBf16>(acc[mt][nt], a0, a1, a2, a3, pb[ks][nt][0][0], pb[ks][nt][0][1]);
-                            mma16816<kBf16>(acc[mt][nt], a0, a1, a2, a3, pb[ks][nt][1][0], pb[ks][nt][1][1]);
-                            if constexpr (kBf16) {
-                                if (p.p_parts > 2)
-                                    mma16816<kBf16>(acc[mt][nt], a0, a1, a2, a3, third[nt][0], third[nt][1]);
-                            }
+                        for (int e = 0; e < 4; ++e) acc[mt][nt][e] += x[e];
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < T::kChunks; c += 2) {
+                    uint32_t r[4];
+                    ldmatrix4_trans(r, v_src + ks * 16 * T::kRow + (((v_chunk + c) ^ v_xor) << 4));
+                    if constexpr (k8) {
+                        // A register holds elements 2g, 2g + 1 of keys 2 t4, 2 t4 + 1: pair the keys.
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t x = __byte_perm(r[2 * h], 0, 0x3120), y = __byte_perm(r[2 * h + 1], 0, 0x3120);
+                            block(c + h, e4m3_f16x2(x), e4m3_f16x2(x >> 16), e4m3_f16x2(y), e4m3_f16x2(y >> 16));
                         }
+                    } else {
+                        block(c / 2, r[0], r[1], r[2], r[3]);
                     }
                 }
             }
         }
-        stage = stage + 1 == S ? 0 : stage + 1;
 
         const bool item_done = at.tile + 1 == at.tiles;
         if (item_done || step + 1 == last) {
-            // Join the warps' states of this item through shared memory, eight query heads at a time.
+            // Join the slices' states of this item through the shared memory of the
+            // stage just read, eight query heads of each part at a time.
             const bool whole = item_done && !head_cut;
             const int kv_head = p.blocks == 1 ? at.hb : at.hb / p.blocks;
             const int head0 = (at.hb - kv_head * p.blocks) * T::kRows;
             const int slot = blockIdx.x * 2 + (head_cut ? 0 : 1);
+            float *const comb0 = reinterpret_cast<float *>(smem + stage * T::kStage);
+            constexpr int kSliceFloats = S * T::kStage / 4;
+            slice_sync();  // every lane has read the stage
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                if (head0 + nt * 8 >= p.group) break;
                 float l0 = sum[nt][0], l1 = sum[nt][1];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) {
@@ -934,37 +957,41 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
                     s_ml[warp][2 * t4 + 1][0] = base[nt][1];
                     s_ml[warp][2 * t4 + 1][1] = l1;
                 }
-                float *const out = comb + (warp * 8 + 2 * t4) * T::kCombStride;
+                float *const out = comb0 + slice * kSliceFloats + (part * 8 + 2 * t4) * T::kCombStride;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    const int d = (mt / (T::VE / 2)) * (8 * T::VE) + g * T::VE + 2 * (mt % (T::VE / 2));
-                    *reinterpret_cast<float2 *>(out + d) = make_float2(acc[mt][nt][0], acc[mt][nt][2]);
-                    *reinterpret_cast<float2 *>(out + T::kCombStride + d) =
-                        make_float2(acc[mt][nt][1], acc[mt][nt][3]);
+                    const int d0 = mt * 16 + (k8 ? 2 * g : g), d1 = k8 ? d0 + 1 : d0 + 8;
+                    out[d0] = acc[mt][nt][0];
+                    out[d1] = acc[mt][nt][2];
+                    out[T::kCombStride + d0] = acc[mt][nt][1];
+                    out[T::kCombStride + d1] = acc[mt][nt][3];
                 }
                 __syncthreads();
-                for (int i = tid; i < 8 * (D / 4); i += kDecodeThreads) {
-                    const int r = i / (D / 4), d = (i % (D / 4)) * 4, head = head0 + nt * 8 + r;
-                    if (head >= p.group) break;
+                for (int i = tid; i < T::kShare * 8 * (D / 4); i += kDecodeThreads) {
+                    const int r = i / (D / 4), d = (i % (D / 4)) * 4, of = r / 8, col = r % 8;
+                    const int in_block = of * (8 * NT) + nt * 8 + col, head = head0 + in_block;
+                    if (head >= p.group) continue;
                     float m = -INFINITY;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][r][0]);
+                    for (int w = 0; w < T::kSlices; ++w) m = fmaxf(m, s_ml[w * T::kShare + of][col][0]);
                     float l = 0.0f;
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        if (s_ml[w][r][1] == 0.0f) continue;  // no keys
-                        const float f = ex2_approx(s_ml[w][r][0] - m);
-                        const float4 y = *reinterpret_cast<const float4 *>(comb + (w * 8 + r) * T::kCombStride + d);
-                        l += s_ml[w][r][1] * f;
+                    for (int w = 0; w < T::kSlices; ++w) {
+                        const float *const ml = s_ml[w * T::kShare + of][col];
+                        if (ml[1] == 0.0f) continue;  // no keys
+                        const float f = ex2_approx(ml[0] - m);
+                        const float4 y =
+                            *reinterpret_cast<const float4 *>(comb0 + w * kSliceFloats + r * T::kCombStride + d);
+                        l += ml[1] * f;
                         x = make_float4(x.x + y.x * f, x.y + y.y * f, x.z + y.z * f, x.w + y.w * f);
                     }
                     if (whole) {
                         finish_quad(p, at.b, kv_head, kv_head * p.group + head, d, x, m, l);
                     } else {
-                        const long long row = static_cast<long long>(slot) * T::kRows + nt * 8 + r;
-                        *reinterpret_cast<float4 *>(p.part_o + row * D + d) = x;
-                        if (d == 0) p.part_ml[row] = make_float2(m, l);
+                        const long long to = static_cast<long long>(slot) * T::kRows + in_block;
+                        *reinterpret_cast<float4 *>(p.part_o + to * D + d) = x;
+                        if (d == 0) p.part_ml[to] = make_float2(m, l);
                     }
                 }
                 __syncthreads();
@@ -972,7 +999,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
             // The CTA in which an item begins says how many CTAs hold parts of it.
             if (tid == 0 && !head_cut) {
                 const long long end = step + (at.tiles - at.tile);  // first tile after the item
-                const int ctas = static_cast<int>((end - 1) / per - blockIdx.x) + 1;
+                const int ctas = static_cast<int>((end - 1) / per) - run + 1;
                 if (p.records_by_item)
                     p.records[static_cast<long long>(at.b) * p.head_blocks + at.hb] =
                         make_int4(at.b, at.hb, ctas, blockIdx.x);
@@ -984,6 +1011,7 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kSmem > 113 * 1024 ? 1 : kC
             head_cut = false;
             fresh = true;
         }
+        stage = stage + 1 == S ? 0 : stage + 1;
         at.advance(p);
     }
 }
@@ -1005,10 +1033,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join(const DecodeParams p,
     const int row = blockIdx.x % rows;
     const int kv_head = rec.y / p.blocks, head = (rec.y - kv_head * p.blocks) * row_stride + row;
     if (head >= p.group) return;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, next_cta = p.by_head ? p.head_blocks : 1;
     // Part 0 is the first CTA's second slot, the others are their CTA's first.
     auto at = [&](int i) {
-        return static_cast<long long>((rec.w + i) * 2 + (i == 0 ? 1 : 0)) * row_stride + row;
+        return static_cast<long long>((rec.w + i * next_cta) * 2 + (i == 0 ? 1 : 0)) * row_stride + row;
     };
     float m = -INFINITY;
     for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, p.part_ml[at(i)].x);
