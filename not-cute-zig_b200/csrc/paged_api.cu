@@ -371,6 +371,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     p.page = fast_div(static_cast<uint32_t>(c.page_size));
     p.scale_log2 = static_cast<float>(static_cast<double>(d.scale) * 1.4426950408889634);
     p.whole_groups = c.page_size % 16 == 0;
+    p.same_strides = p.k_page == p.v_page && p.k_tok == p.v_tok;
     p.q_bf16 = d.q_dtype == NCZ_DTYPE_BF16;
     p.o_dtype = d.o_dtype;
     p.q_vec = aligned(d.q, 8) && d.q_batch_stride % 4 == 0 && d.q_head_stride % 4 == 0;
@@ -401,10 +402,18 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         int s = launch(k, grid, nczp::kDecodeThreads, dev, d.stream, args);
         // Rows of one tile are whole in one CTA: nothing to join.
         if (s != NCZ_SUCCESS || most == 1) return s;
-        int join_rows = static_cast<int>(std::min(group, static_cast<size_t>(rows))), row_stride = rows;
+        // Quads (four elements) per join block: as few as keep the grid within
+        // four blocks an SM, a 128-byte line of a part's row at least.
         const unsigned records = p.records_by_item ? static_cast<unsigned>(items) : grid;
-        void *join_args[3] = {&p, &join_rows, &row_stride};
-        return launch(g_join[dim_index(c.head_dim)], records * join_rows, nczp::kJoinThreads, dev, d.stream,
+        const int total = static_cast<int>(std::min(group, static_cast<size_t>(rows)) * c.head_dim / 4);
+        int quads = 8, join_rows = rows;
+        auto blocks_of = [&](int q) { return (total + q - 1) / q; };
+        while (quads < nczp::kJoinThreads &&
+               static_cast<size_t>(records) * blocks_of(quads) > 4 * static_cast<size_t>(sms))
+            quads *= 2;
+        int per_record = blocks_of(quads);
+        void *join_args[4] = {&p, &join_rows, &quads, &per_record};
+        return launch(g_join[dim_index(c.head_dim)], records * per_record, nczp::kJoinThreads, dev, d.stream,
                       join_args);
     });
 }

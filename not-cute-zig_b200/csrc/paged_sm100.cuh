@@ -334,11 +334,17 @@ struct DecodeParams {
     int batch, group, blocks, head_blocks;  // query heads per K/V head; blocks of them; kv_heads * blocks
     int width_keys, window, num_pages;
     int whole_groups;  // page_size is a multiple of 16: the 16 keys of a group lie in one page
+    int same_strides;  // K's and V's strides are equal
     int by_head;       // every CTA stays with one head block (see paged_decode)
     FastDiv page;
     float scale_log2;
     int records_by_item;
     int q_bf16, o_dtype, q_vec, o_vec, p_parts;
+};
+
+template <bool kValue>
+struct Flag {
+    static constexpr bool value = kValue;
 };
 
 constexpr int kWarps = 4;
@@ -358,7 +364,8 @@ struct Decode {
     static constexpr int kChunks = kRow / 16;         // 16-byte chunks of a row
     static constexpr int kRowsPerCopy = 32 / kChunks; // rows a warp's copy instruction covers
     static constexpr int kCopies = 16 / kRowsPerCopy; // copy instructions of 16 rows
-    static constexpr int KS = kShare * (kRow >= 256 ? 1 : kRow >= 64 ? 2 : 4);  // 16-key groups per step
+    static constexpr int kSwizzles = kRowsPerCopy < 8 ? 8 / kRowsPerCopy : 1;  // different swizzles among them
+    static constexpr int KS = kShare * (kRow >= 256 ? 1 : kRow >= 128 ? 2 : 4);  // 16-key groups per step
     static constexpr int kKeys = 16 * KS;                                       // keys per slice and step
     static constexpr int kSlices = kWarps / kShare;
     static constexpr int kTile = kKeys * kSlices;      // keys per CTA and step
@@ -402,6 +409,22 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// d = a b (16 x 8 x 16), starting a new sum.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    if constexpr (kBf16) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    } else {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    }
+}
 template <bool kBf16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -503,7 +526,7 @@ template <class T>
 __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const DecodeParams p) {
     constexpr int D = T::D, NT = T::NT, KS = T::KS, MT = T::MT, S = T::kStages;
     constexpr bool kBf16 = T::kKv == kBF16, k8 = T::kKv == kE4M3;
-    extern __shared__ __align__(128) char smem[];
+    extern __shared__ __align__(256) char smem[];
     __shared__ long long warp_sums[kWarps];
     __shared__ int s_start[3];
     __shared__ uint32_t s_mask[kWarps][S][T::kMaskWords];
@@ -591,9 +614,15 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
     constexpr int kIds = KS > T::kMaskWords ? KS : T::kMaskWords;
     Cursor<T::kTile> ahead = at;
     long long ahead_left = last - first;
-    int ids[kIds];
+    int ids[kIds];           // page ids, -1 for keys past the end
+    uint32_t in_page[kIds];  // rows in those pages
     const int row = lane / T::kChunks, chunk = lane % T::kChunks;
     const long long k_lane = row * p.k_tok + chunk * 16, v_lane = row * p.v_tok + chunk * 16;
+    const long long k_copy = T::kRowsPerCopy * p.k_tok, v_copy = T::kRowsPerCopy * p.v_tok;
+    uint32_t to[T::kSwizzles];  // where this lane's 16 bytes of a copy go, from the copy's first row
+#pragma unroll
+    for (int i = 0; i < T::kSwizzles; ++i)
+        to[i] = ring + row * T::kRow + ((chunk ^ chunk_xor<T::kRow>(i * T::kRowsPerCopy + row)) << 4);
     auto first_key = [&](const Cursor<T::kTile> &c) {  // of this warp's slice, a multiple of 16
         return static_cast<uint32_t>(c.lo & ~15) + static_cast<uint32_t>(c.tile) * T::kTile + slice * T::kKeys;
     };
@@ -604,14 +633,18 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
         if (p.whole_groups) {
             // One id per group of 16 keys, the same in every lane.
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
-                ids[i] = key0 + i * 16 < hi ? __ldg(table + p.page.div(key0 + i * 16)) : -1;
+            for (int i = 0; i < KS; ++i) {
+                const uint32_t key = key0 + i * 16, col = p.page.div(key);
+                in_page[i] = key - col * p.page.d;
+                ids[i] = key < hi ? __ldg(table + col) : -1;
+            }
         } else {
             // Key i * 32 + lane's id.
 #pragma unroll
             for (int i = 0; i < T::kMaskWords; ++i) {
-                const uint32_t key = key0 + i * 32 + lane;
-                ids[i] = i * 32 + lane < T::kKeys && key < hi ? __ldg(table + p.page.div(key)) : -1;
+                const uint32_t key = key0 + i * 32 + lane, col = p.page.div(key);
+                in_page[i] = key - col * p.page.d;
+                ids[i] = i * 32 + lane < T::kKeys && key < hi ? __ldg(table + col) : -1;
             }
         }
     };
@@ -620,7 +653,8 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
             const int kv_head = p.blocks == 1 ? ahead.hb : ahead.hb / p.blocks;
             const char *const kb = p.k + kv_head * p.k_head, *const vb = p.v + kv_head * p.v_head;
             const uint32_t key0 = first_key(ahead), lo = ahead.lo, hi = ahead.hi;
-            const uint32_t k_dst = ring + stage * T::kStage, v_dst = k_dst + T::kKeys * T::kRow;
+            const uint32_t at_stage = stage * T::kStage;
+            constexpr uint32_t kV = T::kKeys * T::kRow;  // V's rows follow K's
             uint32_t mask[T::kMaskWords];
             if (p.whole_groups) {
 #pragma unroll
@@ -629,55 +663,66 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t key = key0 + ks * 16;
                     if (static_cast<uint32_t>(ids[ks]) < static_cast<uint32_t>(p.num_pages)) {  // hence key < hi
-                        uint32_t m = hi - key < 16 ? (1u << (hi - key)) - 1 : 0xFFFFu;
+                        uint32_t m = 0xFFFFu;
+                        if (hi - key < 16) m = (1u << (hi - key)) - 1;
                         if (key < lo) m &= lo - key < 16 ? ~((1u << (lo - key)) - 1) : 0u;
                         mask[ks / 2] |= m << (ks % 2 * 16);
-                        const uint32_t in_page = key - p.page.div(key) * p.page.d;
-                        const char *k_src = kb + (ids[ks] * p.k_page + in_page * p.k_tok) + k_lane;
-                        const char *v_src = vb + (ids[ks] * p.v_page + in_page * p.v_tok) + v_lane;
+                        const long long k_off = ids[ks] * p.k_page + in_page[ks] * p.k_tok;
+                        const long long v_off = p.same_strides ? k_off : ids[ks] * p.v_page + in_page[ks] * p.v_tok;
+                        const char *k_src = kb + k_off + k_lane, *v_src = vb + v_off + v_lane;
+                        if (m == 0xFFFFu) {
 #pragma unroll
-                        for (int j = 0; j < T::kCopies; ++j) {
-                            const uint32_t r = ks * 16 + j * T::kRowsPerCopy + row;
-                            const uint32_t to = r * T::kRow + ((chunk ^ chunk_xor<T::kRow>(r)) << 4);
-                            if ((ks * T::kCopies + j) % T::kShare == part) {
-                                if (m == 0xFFFFu) {
-                                    copy16(k_dst + to, k_src);
-                                    copy16(v_dst + to, v_src);
-                                } else {
-                                    const uint32_t bytes = ((m >> (r & 15)) & 1) * 16;
-                                    copy16(k_dst + to, k_src, bytes);
-                                    copy16(v_dst + to, v_src, bytes);
+                            for (int j = 0; j < T::kCopies; ++j) {
+                                const uint32_t dst = to[j % T::kSwizzles] + at_stage +
+                                                     (ks * 16 + j * T::kRowsPerCopy) * T::kRow;
+                                if ((ks * T::kCopies + j) % T::kShare == part) {
+                                    copy16(dst, k_src);
+                                    copy16(dst + kV, v_src);
                                 }
+                                k_src += k_copy;
+                                v_src += v_copy;
                             }
-                            k_src += T::kRowsPerCopy * p.k_tok;
-                            v_src += T::kRowsPerCopy * p.v_tok;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < T::kCopies; ++j) {
+                                const uint32_t dst = to[j % T::kSwizzles] + at_stage +
+                                                     (ks * 16 + j * T::kRowsPerCopy) * T::kRow;
+                                const uint32_t bytes = ((m >> (j * T::kRowsPerCopy + row)) & 1) * 16;
+                                if ((ks * T::kCopies + j) % T::kShare == part) {
+                                    copy16(dst, k_src, bytes);
+                                    copy16(dst + kV, v_src, bytes);
+                                }
+                                k_src += k_copy;
+                                v_src += v_copy;
+                            }
                         }
                     }
                 }
             } else {
-                long long k_off[T::kMaskWords], v_off[T::kMaskWords];
 #pragma unroll
                 for (int i = 0; i < T::kMaskWords; ++i) {
-                    const uint32_t key = key0 + i * 32 + lane;
-                    const bool ok = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(p.num_pages) && key >= lo;
-                    const uint32_t in_page = ok ? key - p.page.div(key) * p.page.d : 0;
-                    k_off[i] = ok ? ids[i] * p.k_page + in_page * p.k_tok : -1;
-                    v_off[i] = ok ? ids[i] * p.v_page + in_page * p.v_tok : -1;
+                    const bool ok = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(p.num_pages) &&
+                                    key0 + i * 32 + lane >= lo;
                     mask[i] = __ballot_sync(~0u, ok);
+                    if (!ok) ids[i] = 0, in_page[i] = 0;  // a row of the cache, of which 0 bytes are read
                 }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    if (((mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu) == 0) continue;
+                    const uint32_t m = (mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu;
+                    if (m == 0) continue;
 #pragma unroll
                     for (int j = 0; j < T::kCopies; ++j) {
                         if ((ks * T::kCopies + j) % T::kShare != part) continue;
-                        const uint32_t r = ks * 16 + j * T::kRowsPerCopy + row;
-                        const uint32_t to = r * T::kRow + ((chunk ^ chunk_xor<T::kRow>(r)) << 4);
-                        const long long ko = __shfl_sync(~0u, k_off[ks / 2], r & 31);
-                        const long long vo = __shfl_sync(~0u, v_off[ks / 2], r & 31);
-                        const uint32_t bytes = ko >= 0 ? 16 : 0;
-                        copy16(k_dst + to, kb + (ko >= 0 ? ko + chunk * 16 : 0), bytes);
-                        copy16(v_dst + to, vb + (vo >= 0 ? vo + chunk * 16 : 0), bytes);
+                        const uint32_t r = j * T::kRowsPerCopy + row;
+                        const int id = __shfl_sync(~0u, ids[ks / 2], (ks % 2 * 16 + r) & 31);
+                        const uint32_t in = __shfl_sync(~0u, in_page[ks / 2], (ks % 2 * 16 + r) & 31);
+                        const long long k_off = id * p.k_page + in * p.k_tok;
+                        const long long v_off = p.same_strides ? k_off : id * p.v_page + in * p.v_tok;
+                        const uint32_t dst = to[j % T::kSwizzles] + at_stage +
+                                             (ks * 16 + j * T::kRowsPerCopy) * T::kRow;
+                        const uint32_t bytes = ((m >> r) & 1) * 16;
+                        copy16(dst, kb + k_off + chunk * 16, bytes);
+                        copy16(dst + kV, vb + v_off + chunk * 16, bytes);
                     }
                 }
             }
@@ -693,32 +738,32 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
     };
 
     look_up();
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < S - 1; ++s) produce(s);
 
     // ---- consumer side.  Scores S^T = K Q^T (keys as rows), O^T = V^T P^T (head_dim as rows).
     float acc[MT][NT][4];  // O^T: rows g and g + 8 of block mt, query heads 2 t4 and 2 t4 + 1
     float base[NT][2], sum[NT][2];
     uint32_t qf[D / 16][NT][2];
-    float q_up[NT][2];  // power of two taken out of a query head's elements (bf16 q against an e4m3 cache)
+    float f[NT][2];  // what turns a score into log2 units, above 0 (the sign is in qf)
     bool fresh = true;
     bool head_cut = at.tile != 0;  // this CTA's first item began in another CTA
     int stage = 0;
-    float scale = 0.0f;
     // Rows and chunks of this lane's ldmatrix addresses: matrices 0..3 of K are
     // (keys 0-7 | 8-15) x (chunk, chunk + 1); those of V (trans) the same for e4m3 and
     // (chunk, chunk + 1) x (keys 0-7 | 8-15) for 16-bit types.
     const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk = lane >> 4;
     const uint32_t v_row = k8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_chunk = k8 ? k_chunk : (lane >> 3) & 1;
-    const uint32_t k_at = k_row * T::kRow, k_xor = chunk_xor<T::kRow>(k_row);
-    const uint32_t v_at = v_row * T::kRow, v_xor = chunk_xor<T::kRow>(v_row);
+    // Address of chunk c: these ^ (c << 4) (rows and stages start on multiples of kRow).
+    const uint32_t k_at = ring + k_row * T::kRow + ((k_chunk ^ chunk_xor<T::kRow>(k_row)) << 4);
+    const uint32_t v_at = ring + T::kKeys * T::kRow + v_row * T::kRow + ((v_chunk ^ chunk_xor<T::kRow>(v_row)) << 4);
 
     for (long long step = first; step < last; ++step) {
         if (fresh) {
             fresh = false;
             const int kv_head = p.blocks == 1 ? at.hb : at.hb / p.blocks;
             const int head0 = (at.hb - kv_head * p.blocks) * T::kRows + part * (8 * NT);  // of the group
-            scale = p.scale_log2 * (k8 && p.k_scale != nullptr ? __ldg(p.k_scale + kv_head) : 1.0f);
+            const float scale = p.scale_log2 * (k8 && p.k_scale != nullptr ? __ldg(p.k_scale + kv_head) : 1.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int head = head0 + nt * 8 + g;
@@ -739,8 +784,8 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                             w[j] = q[d] | (static_cast<uint32_t>(q[d + 1]) << 16);
                     }
                 }
+                float up = 1.0f;
                 if constexpr (k8) {
-                    float up = 1.0f;
                     if (p.q_bf16) {
                         // bf16 spans more than f16: take a power of two out of the row, so
                         // that its largest element lies in [1, 2); what f16 then rounds is below
@@ -750,8 +795,8 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float2 f = unpack16<true>(qf[kk][nt][j]);
-                                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                                const float2 x = unpack16<true>(qf[kk][nt][j]);
+                                top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                             }
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
@@ -764,13 +809,22 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float2 f = unpack16<true>(qf[kk][nt][j]);
-                                qf[kk][nt][j] = ncz::pack_f16x2(f.x * down, f.y * down);
+                                const float2 x = unpack16<true>(qf[kk][nt][j]);
+                                qf[kk][nt][j] = ncz::pack_f16x2(x.x * down, x.y * down);
                             }
                     }
-                    q_up[nt][0] = __shfl_sync(~0u, up, (2 * t4) * 4);
-                    q_up[nt][1] = __shfl_sync(~0u, up, (2 * t4 + 1) * 4);
                 }
+                if (scale < 0.0f) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) qf[kk][nt][j] ^= 0x80008000u;
+                }
+                // Not 0: masked scores stay -infinity times it.  1e-35 of any finite score is 0 beside a 1.
+                up *= fabsf(scale);
+                up = up == 0.0f ? 1e-35f : up;
+                f[nt][0] = __shfl_sync(~0u, up, (2 * t4) * 4);
+                f[nt][1] = __shfl_sync(~0u, up, (2 * t4 + 1) * 4);
                 base[nt][0] = base[nt][1] = -INFINITY;
                 sum[nt][0] = sum[nt][1] = 0.0f;
 #pragma unroll
@@ -788,55 +842,74 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
 #pragma unroll
         for (int i = 0; i < T::kMaskWords; ++i) any |= mask[i] = s_mask[warp][stage][i];
         if (any != 0) {
-            const uint32_t k_src = ring + stage * T::kStage + k_at;
-            const uint32_t v_src = ring + stage * T::kStage + T::kKeys * T::kRow + v_at;
+            const uint32_t k_src = k_at + stage * T::kStage, v_src = v_at + stage * T::kStage;
             float s[KS][NT][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[ks][nt][e] = 0.0f;
-#pragma unroll
                 for (int c = 0; c < T::kChunks; c += 2) {
                     uint32_t r[4];
-                    ldmatrix4(r, k_src + ks * 16 * T::kRow + (((k_chunk + c) ^ k_xor) << 4));
+                    ldmatrix4(r, (k_src ^ (c << 4)) + ks * 16 * T::kRow);
                     if constexpr (k8) {
                         // A chunk is 16 elements: two products.
+                        uint32_t a[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            a[i] = e4m3_f16x2(r[i]);
+                            a[4 + i] = e4m3_f16x2(r[i] >> 16);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma16816<false>(s[ks][nt], e4m3_f16x2(r[0]), e4m3_f16x2(r[1]), e4m3_f16x2(r[0] >> 16),
-                                            e4m3_f16x2(r[1] >> 16), qf[c][nt][0], qf[c][nt][1]);
-                            mma16816<false>(s[ks][nt], e4m3_f16x2(r[2]), e4m3_f16x2(r[3]), e4m3_f16x2(r[2] >> 16),
-                                            e4m3_f16x2(r[3] >> 16), qf[c + 1][nt][0], qf[c + 1][nt][1]);
+                            if (c == 0)
+                                mma16816_new<false>(s[ks][nt], a[0], a[1], a[4], a[5], qf[c][nt][0], qf[c][nt][1]);
+                            else
+                                mma16816<false>(s[ks][nt], a[0], a[1], a[4], a[5], qf[c][nt][0], qf[c][nt][1]);
+                            mma16816<false>(s[ks][nt], a[2], a[3], a[6], a[7], qf[c + 1][nt][0], qf[c + 1][nt][1]);
                         }
                     } else {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma16816<kBf16>(s[ks][nt], r[0], r[1], r[2], r[3], qf[c / 2][nt][0], qf[c / 2][nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (c == 0)
+                                mma16816_new<kBf16>(s[ks][nt], r[0], r[1], r[2], r[3], qf[0][nt][0], qf[0][nt][1]);
+                            else
+                                mma16816<kBf16>(s[ks][nt], r[0], r[1], r[2], r[3], qf[c / 2][nt][0], qf[c / 2][nt][1]);
+                        }
                     }
                 }
             }
-            // Scores in log2 units; keys outside the mask -infinity (their rows may be
-            // zeros or, where a whole group is absent, an older step's).
-            bool grow = false;
-            float top[NT][2];
+            // Keys outside the mask: -infinity (their rows may be zeros or, where a
+            // whole group is absent, an older step's).
+            uint32_t every = mask[0];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float f0 = k8 ? scale * q_up[nt][0] : scale, f1 = k8 ? scale * q_up[nt][1] : scale;
-                top[nt][0] = top[nt][1] = -INFINITY;
+            for (int i = 1; i < T::kMaskWords; ++i) every &= mask[i];
+            if (every != (T::kKeys < 32 ? (1u << (T::kKeys & 31)) - 1 : ~0u)) {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const bool in0 = (mask[ks / 2] >> ((ks * 16 + g) & 31)) & 1;
                     const bool in1 = (mask[ks / 2] >> ((ks * 16 + 8 + g) & 31)) & 1;
-                    float(&x)[4] = s[ks][nt];
-                    x[0] = in0 ? x[0] * f0 : -INFINITY;
-                    x[1] = in0 ? x[1] * f1 : -INFINITY;
-                    x[2] = in1 ? x[2] * f0 : -INFINITY;
-                    x[3] = in1 ? x[3] * f1 : -INFINITY;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float(&x)[4] = s[ks][nt];
+                        x[0] = in0 ? x[0] : -INFINITY;
+                        x[1] = in0 ? x[1] : -INFINITY;
+                        x[2] = in1 ? x[2] : -INFINITY;
+                        x[3] = in1 ? x[3] : -INFINITY;
+                    }
+                }
+            }
+            bool grow = false;
+            float top[NT][2];  // in log2 units
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const float(&x)[4] = s[ks][nt];
                     top[nt][0] = fmaxf(top[nt][0], fmaxf(x[0], x[2]));
                     top[nt][1] = fmaxf(top[nt][1], fmaxf(x[1], x[3]));
                 }
+                top[nt][0] *= f[nt][0];
+                top[nt][1] *= f[nt][1];
                 grow |= top[nt][0] > base[nt][0] + kTop || top[nt][1] > base[nt][1] + kTop;
             }
             if (__any_sync(~0u, grow)) {
@@ -849,13 +922,13 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                         m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
                         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
                         const float to = fmaxf(base[nt][j], m - kLift);
-                        const float f = base[nt][j] == -INFINITY ? 0.0f : ex2_approx(base[nt][j] - to);
+                        const float down = base[nt][j] == -INFINITY ? 0.0f : ex2_approx(base[nt][j] - to);
                         base[nt][j] = to;
-                        sum[nt][j] *= f;
+                        sum[nt][j] *= down;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            acc[mt][nt][j] *= f;
-                            acc[mt][nt][j + 2] *= f;
+                            acc[mt][nt][j] *= down;
+                            acc[mt][nt][j + 2] *= down;
                         }
                     }
             }
@@ -866,16 +939,17 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     float(&x)[4] = s[ks][nt];
-                    x[0] = ex2_approx(x[0] - m0);
-                    x[1] = ex2_approx(x[1] - m1);
-                    x[2] = ex2_approx(x[2] - m0);
-                    x[3] = ex2_approx(x[3] - m1);
+                    x[0] = ex2_approx(fmaf(x[0], f[nt][0], -m0));
+                    x[1] = ex2_approx(fmaf(x[1], f[nt][1], -m1));
+                    x[2] = ex2_approx(fmaf(x[2], f[nt][0], -m0));
+                    x[3] = ex2_approx(fmaf(x[3], f[nt][1], -m1));
                     sum[nt][0] += x[0] + x[2];
                     sum[nt][1] += x[1] + x[3];
                 }
             }
             // P^T fragments in 16-bit parts: each takes the rounded value and leaves the rest to the next.
-            auto next_part = [&](int ks, int nt, uint32_t (&b)[2]) {
+            uint32_t b[KS][NT][kBf16 ? 3 : 2][2];
+            auto next_part = [&](int ks, int nt, int i) {
                 float(&x)[4] = s[ks][nt];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -883,53 +957,87 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                     const float2 back = unpack16<kBf16>(w);
                     x[2 * h] -= back.x;
                     x[2 * h + 1] -= back.y;
-                    b[h] = transpose8x8(w);
+                    b[ks][nt][i][h] = transpose8x8(w);
                 }
             };
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if constexpr (KS > 1)
-                    if (((mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu) == 0) continue;  // V's rows are not there
-                uint32_t b[3][NT][2];
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    next_part(ks, nt, b[0][nt]);
-                    next_part(ks, nt, b[1][nt]);
+                    next_part(ks, nt, 0);
+                    next_part(ks, nt, 1);
                     if constexpr (kBf16) {
-                        if (p.p_parts > 2) next_part(ks, nt, b[2][nt]);
+                        if (p.p_parts > 2) next_part(ks, nt, 2);
                     }
                 }
-                // The products of one group are summed apart and then added: the matrix unit's own
-                // additions cut off below 2^-24 of the sum, always downwards in magnitude.
-                auto block = [&](int mt, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            // The products of a step are summed apart, small parts first, and then added: the
+            // matrix unit's own additions cut off below 2^-24 of the sum, always downwards in
+            // magnitude, which over a whole row would leave 1e-6 of it.
+            auto block = [&](int ks, int nt, float (&x)[4], bool fresh_sum, uint32_t a0, uint32_t a1, uint32_t a2,
+                             uint32_t a3) {
+                const auto &w = b[ks][nt];
+                if (fresh_sum)
+                    mma16816_new<kBf16>(x, a0, a1, a2, a3, w[1][0], w[1][1]);
+                else
+                    mma16816<kBf16>(x, a0, a1, a2, a3, w[1][0], w[1][1]);
+                if constexpr (kBf16) {
+                    if (p.p_parts > 2) mma16816<kBf16>(x, a0, a1, a2, a3, w[2][0], w[2][1]);
+                }
+                mma16816<kBf16>(x, a0, a1, a2, a3, w[0][0], w[0][1]);
+            };
+            // Groups without a key are left out: their V rows are not there.
+            uint32_t groups = 0;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if constexpr (kBf16) {
-                            if (p.p_parts > 2) mma16816<kBf16>(x, a0, a1, a2, a3, b[2][nt][0], b[2][nt][1]);
-                        }
-                        mma16816<kBf16>(x, a0, a1, a2, a3, b[1][nt][0], b[1][nt][1]);
-                        mma16816<kBf16>(x, a0, a1, a2, a3, b[0][nt][0], b[0][nt][1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[mt][nt][e] += x[e];
-                    }
-                };
+            for (int ks = 0; ks < KS; ++ks)
+                groups |= (((mask[ks / 2] >> (ks % 2 * 16)) & 0xFFFFu) != 0 ? 1u : 0u) << ks;
+            auto products = [&](auto all_groups) {
 #pragma unroll
                 for (int c = 0; c < T::kChunks; c += 2) {
-                    uint32_t r[4];
-                    ldmatrix4_trans(r, v_src + ks * 16 * T::kRow + (((v_chunk + c) ^ v_xor) << 4));
-                    if constexpr (k8) {
-                        // A register holds elements 2g, 2g + 1 of keys 2 t4, 2 t4 + 1: pair the keys.
+                    float x[k8 ? 2 : 1][NT][4];
+                    if constexpr (!decltype(all_groups)::value) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t x = __byte_perm(r[2 * h], 0, 0x3120), y = __byte_perm(r[2 * h + 1], 0, 0x3120);
-                            block(c + h, e4m3_f16x2(x), e4m3_f16x2(x >> 16), e4m3_f16x2(y), e4m3_f16x2(y >> 16));
-                        }
-                    } else {
-                        block(c / 2, r[0], r[1], r[2], r[3]);
+                        for (int h = 0; h < (k8 ? 2 : 1); ++h)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[h][nt][e] = 0.0f;
                     }
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        if constexpr (!decltype(all_groups)::value) {
+                            if (!((groups >> ks) & 1)) continue;
+                        }
+                        const bool fresh_sum = decltype(all_groups)::value && ks == 0;
+                        uint32_t r[4];
+                        ldmatrix4_trans(r, (v_src ^ (c << 4)) + ks * 16 * T::kRow);
+                        if constexpr (k8) {
+                            // A register holds elements 2g, 2g + 1 of keys 2 t4, 2 t4 + 1: pair the keys.
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t lo = __byte_perm(r[2 * h], 0, 0x3120);
+                                const uint32_t hi = __byte_perm(r[2 * h + 1], 0, 0x3120);
+                                const uint32_t a0 = e4m3_f16x2(lo), a1 = e4m3_f16x2(lo >> 16);
+                                const uint32_t a2 = e4m3_f16x2(hi), a3 = e4m3_f16x2(hi >> 16);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) block(ks, nt, x[h][nt], fresh_sum, a0, a1, a2, a3);
+                            }
+                        } else {
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) block(ks, nt, x[0][nt], fresh_sum, r[0], r[1], r[2], r[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < (k8 ? 2 : 1); ++h)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[k8 ? c + h : c / 2][nt][e] += x[h][nt][e];
                 }
-            }
+            };
+            if (groups == (1u << KS) - 1)
+                products(Flag<true>());
+            else
+                products(Flag<false>());
         }
 
         const bool item_done = at.tile + 1 == at.tiles;
@@ -1018,55 +1126,63 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
 
 constexpr int kJoinThreads = 256;
 
-// Joins the parts of one query head's row: block (record, row).  D / 4 threads
-// take one part's row together, kJoinThreads / (D / 4) parts at a time.
+// Joins the parts of a row.  A thread takes four elements of one query head
+// (a quad) over every kJoinThreads / quads-th part; block i works on quads
+// [i % per_record * quads, ...) of record i / per_record.  Few records take few
+// quads per block, so that many threads share the parts of each; many take up
+// to a whole item's rows, so that the grid stays within one wave of blocks.
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_join(const DecodeParams p, int rows, int row_stride) {
-    constexpr int kLanes = D / 4, kSubs = kJoinThreads / kLanes;
-    __shared__ float s_max[kJoinThreads / 32];
-    __shared__ float s_sum[kSubs];
-    __shared__ float4 s_o[kSubs][kLanes];
+__global__ void __launch_bounds__(kJoinThreads)
+    paged_join(const DecodeParams p, int rows, int quads, int per_record) {
+    __shared__ float4 s_o[kJoinThreads / 32][32];
+    __shared__ float2 s_ml[kJoinThreads / 32][32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 rec = p.records[blockIdx.x / rows];
+    const int4 rec = p.records[blockIdx.x / per_record];
     const int n = rec.z;
     if (n <= 1) return;
-    const int row = blockIdx.x % rows;
-    const int kv_head = rec.y / p.blocks, head = (rec.y - kv_head * p.blocks) * row_stride + row;
-    if (head >= p.group) return;
-    const int tid = threadIdx.x, next_cta = p.by_head ? p.head_blocks : 1;
-    // Part 0 is the first CTA's second slot, the others are their CTA's first.
-    auto at = [&](int i) {
-        return static_cast<long long>((rec.w + i * next_cta) * 2 + (i == 0 ? 1 : 0)) * row_stride + row;
-    };
-    float m = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, p.part_ml[at(i)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if ((tid & 31) == 0) s_max[tid >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, s_max[w]);
-    const int sub = tid / kLanes, q = tid % kLanes;
-    float l = 0.0f;
+    const int tid = threadIdx.x, lane = tid & 31, next_cta = p.by_head ? p.head_blocks : 1;
+    const int sub = tid / quads, subs = kJoinThreads / quads;
+    const int quad = (blockIdx.x % per_record) * quads + tid % quads;
+    const int row = quad / (D / 4), d = quad % (D / 4) * 4;
+    const int kv_head = rec.y / p.blocks, head = (rec.y - kv_head * p.blocks) * rows + row;
+    const bool live = row < rows && head < p.group;
+    float m = -INFINITY, l = 0.0f;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // (m, l, x) += (m2, l2, y), both relative to their own maximum; l = 0: no keys.
+    auto add = [&](float m2, float l2, float4 y) {
+        const float to = fmaxf(m, m2);
+        const float a = l == 0.0f ? 0.0f : ex2_approx(m - to), b = l2 == 0.0f ? 0.0f : ex2_approx(m2 - to);
+        m = to;
+        l = l * a + l2 * b;
+        x = make_float4(x.x * a + y.x * b, x.y * a + y.y * b, x.z * a + y.z * b, x.w * a + y.w * b);
+    };
+    if (live) {
 #pragma unroll 4
-    for (int i = sub; i < n; i += kSubs) {
-        const float2 ml = p.part_ml[at(i)];
-        const float4 y = *reinterpret_cast<const float4 *>(p.part_o + at(i) * D + q * 4);
-        const float f = ml.y == 0.0f ? 0.0f : ex2_approx(ml.x - m);  // 0: no keys
-        l += ml.y * f;
-        x = make_float4(x.x + y.x * f, x.y + y.y * f, x.z + y.z * f, x.w + y.w * f);
+        for (int i = sub; i < n; i += subs) {
+            // Part 0 is the first CTA's second slot, the others are their CTA's first.
+            const long long at = static_cast<long long>((rec.w + i * next_cta) * 2 + (i == 0 ? 1 : 0)) * rows + row;
+            const float2 ml = p.part_ml[at];
+            add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part_o + at * D + d));
+        }
     }
-    s_o[sub][q] = x;
-    if (q == 0) s_sum[sub] = l;
-    __syncthreads();
-    if (sub != 0) return;
-    for (int s = 1; s < kSubs; ++s) {
-        const float4 y = s_o[s][q];
-        l += s_sum[s];
-        x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+    // Threads of one quad: first within the warp, then across warps.
+    for (int o = quads; o < 32; o <<= 1) {
+        const float m2 = __shfl_xor_sync(~0u, m, o), l2 = __shfl_xor_sync(~0u, l, o);
+        const float4 y = make_float4(__shfl_xor_sync(~0u, x.x, o), __shfl_xor_sync(~0u, x.y, o),
+                                     __shfl_xor_sync(~0u, x.z, o), __shfl_xor_sync(~0u, x.w, o));
+        add(m2, l2, y);
     }
-    finish_quad(p, rec.x, kv_head, kv_head * p.group + head, q * 4, x, m, l);
+    if (subs > 1) {
+        s_o[tid >> 5][lane] = x;
+        s_ml[tid >> 5][lane] = make_float2(m, l);
+        __syncthreads();
+        if (tid >= quads) return;
+        // With quads >= 32 a warp holds one part's share of 32 quads: the next share is quads / 32 warps on.
+        const int stride = quads < 32 ? 1 : quads / 32;
+        for (int w = (tid >> 5) + stride; w < kJoinThreads / 32; w += stride)
+            add(s_ml[w][lane].x, s_ml[w][lane].y, s_o[w][lane]);
+    }
+    if (live) finish_quad(p, rec.x, kv_head, kv_head * p.group + head, d, x, m, l);
 }
 
 }  // namespace nczp
