@@ -20,6 +20,8 @@ constexpr int kMaxDevices = 64;
 constexpr size_t kMaxInt = 0x7FFFFFFF;
 constexpr size_t kMaxStride = size_t(1) << 40;  // elements; offsets then stay far inside 64 bits
 
+constexpr size_t kPlanClusters = 16, kSlotsPerCluster = 4096;
+
 std::mutex g_mu;
 int g_sms[kMaxDevices];
 
@@ -242,9 +244,14 @@ int ncz_paged_plan(const ncz_paged_plan_desc *desc) {
     p.width = static_cast<int>(d.table_width);
     p.free_capacity = static_cast<int>(d.free_capacity);
     p.page = fast_div(static_cast<uint32_t>(d.page_size));
+    // A cluster per 4096 slots, up to what an SM count of 148 holds at once, unless outputs are
+    // in place of inputs that another cluster may not have read.
+    const bool in_place = d.held == d.seq_lens || d.free_count == d.left;
+    const unsigned clusters =
+        in_place ? 1u : static_cast<unsigned>(std::min<size_t>(kPlanClusters, 1 + d.slot_capacity / kSlotsPerCluster));
     return on_device(d.device, [&](int dev) {
         void *args[1] = {&p};
-        return launch(g_plan, nczp::kPlanCluster, nczp::kPlanThreads, dev, d.stream, args);
+        return launch(g_plan, nczp::kPlanCluster * clusters, nczp::kPlanThreads, dev, d.stream, args);
     });
 }
 
@@ -282,9 +289,9 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
     p.cv_head = static_cast<long long>(c.v_head_stride) * el;
     p.tokens = static_cast<long long>(d.tokens);
     p.num_slots = static_cast<long long>(c.num_pages) * static_cast<long long>(c.page_size);
-    p.chunks = static_cast<int>(c.kv_heads * c.head_dim / 8);
-    p.head_chunks = static_cast<int>(c.head_dim / 8);
-    p.group = std::max(1, 2 * nczp::kAppendThreads / p.chunks);
+    p.head_pieces = static_cast<int>(c.head_dim / nczp::kAppendPiece);
+    p.pieces = static_cast<int>(c.kv_heads) * p.head_pieces;
+    p.group = std::max(1, nczp::kAppendThreads / p.pieces);
     p.vec = aligned(d.k, 16) && aligned(d.v, 16) && p.k_tok % 16 == 0 && p.k_head % 16 == 0 && p.v_tok % 16 == 0 &&
             p.v_head % 16 == 0;
     p.page_size = static_cast<uint32_t>(c.page_size);

@@ -27,6 +27,12 @@ struct FastDiv {
     __device__ __forceinline__ uint32_t div(uint32_t n) const { return (n + __umulhi(n, mul)) >> shift; }
 };
 
+// A number that a generic lambda takes at compile time.
+template <auto kValue>
+struct Constant {
+    static constexpr auto value = kValue;
+};
+
 // ---------------------------------------------------------------- plan
 
 struct PlanParams {
@@ -41,9 +47,8 @@ struct PlanParams {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCluster = 8;
-constexpr int kPlanPer = 4;                                // requests a thread scans per round
-constexpr int kPlanRound = kPlanThreads * kPlanPer;        // requests per round
-constexpr int kPlanSmem = kPlanRound * 4 * sizeof(int);    // start, first page, held, flags
+constexpr int kPlanRound = kPlanThreads * kPlanCluster;  // requests per round: one a thread
+constexpr int kPlanSmem = kPlanRound * sizeof(int4);
 
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -54,136 +59,152 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 
-// Exclusive prefix of (a, b) over the block's threads, and the block totals.
-__device__ __forceinline__ void block_scan2(long long &a, long long &b, long long &total_a, long long &total_b,
-                                            long long (*warp_sums)[2]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const long long own_a = a, own_b = b;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long xa = __shfl_up_sync(~0u, a, o), xb = __shfl_up_sync(~0u, b, o);
-        if (lane >= o) {
-            a += xa;
-            b += xb;
-        }
-    }
-    if (lane == 31) {
-        warp_sums[warp][0] = a;
-        warp_sums[warp][1] = b;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        long long wa = lane < warps ? warp_sums[lane][0] : 0, wb = lane < warps ? warp_sums[lane][1] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long xa = __shfl_up_sync(~0u, wa, o), xb = __shfl_up_sync(~0u, wb, o);
-            if (lane >= o) {
-                wa += xa;
-                wb += xb;
-            }
-        }
-        if (lane < warps) {
-            warp_sums[lane][0] = wa;
-            warp_sums[lane][1] = wb;
-        }
-    }
-    __syncthreads();
-    total_a = warp_sums[warps - 1][0];
-    total_b = warp_sums[warps - 1][1];
-    a += (warp > 0 ? warp_sums[warp - 1][0] : 0) - own_a;
-    b += (warp > 0 ? warp_sums[warp - 1][1] : 0) - own_b;
-    __syncthreads();
+// The address, in the cluster's window, of `addr` of CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, int x, int y) {
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, long long x, long long y) {
+    asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr), "l"(x), "l"(y) : "memory");
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, const int4 &x) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                 : "memory");
 }
 
-// Last i in [0, n) with start[i] <= x (start is ascending, start[0] <= x).
-__device__ __forceinline__ int last_at_most(const int *start, int n, int x) {
-    int lo = 0, hi = n;  // start[lo] <= x; hi == n or start[hi] > x
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= x)
-            lo = mid;
-        else
-            hi = mid;
+// Last i in [0, n) with start[4 i] <= x (ascending, start[0] <= x), by `bits`
+// halvings of [0, 2^bits).
+__device__ __forceinline__ int last_at_most(const int *start, int n, int bits, int x) {
+    int r = 0;
+    for (int step = bits > 0 ? 1 << (bits - 1) : 0; step > 0; step >>= 1) {
+        const int at = r + step;
+        if (at < n && start[4 * at] <= x) r = at;
     }
-    return lo;
+    return r;
 }
 
-// One cluster of 8 CTAs.  Per round of 4096 requests every CTA scans all of
-// them itself (32 KB of lengths from L2, no exchange between CTAs), keeps
-// the round's prefixes in shared memory, and then writes its share of the
-// slots and table entries, finding each one's request by binary search.  The
-// cluster barrier between reading a round's lengths and writing is what lets
-// seq_lens be held, and left be free_count, in place.
+// Clusters of 8 CTAs.  Per round of 8192 requests every thread of a cluster
+// takes one, the CTAs scan theirs, exchange their totals, and write the prefixes
+// of all requests into every CTA's shared memory.  Then each CTA writes its
+// share of the round's slots and table entries, finding an entry's request by
+// binary search, so that one long prompt is shared by all CTAs too.  The cluster
+// barriers between reading a round's lengths and writing are what lets seq_lens
+// be held, and left be free_count, in place.  Where neither is, several clusters
+// do the same and share the slots and entries (PlanParams; paged_api.cu).
 __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThreads, 1) paged_plan(const PlanParams p) {
-    extern __shared__ int plan_smem[];
-    int *const s_start = plan_smem;              // new tokens before the request, within the round (clamped)
-    int *const s_first = plan_smem + kPlanRound; // pages asked for before it, within the round (clamped)
-    int *const s_held = plan_smem + 2 * kPlanRound;
-    int *const s_have = plan_smem + 3 * kPlanRound;  // pages held; -1 = refused
+    extern __shared__ __align__(16) char plan_smem[];
+    // Of a round's requests: new tokens before it (clamped), pages asked for before it (clamped),
+    // tokens held, pages held (-1 = refused).
+    int4 *const s_req = reinterpret_cast<int4 *>(plan_smem);
     __shared__ long long warp_sums[32][2];
-    const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x;
-    const int all = rank * kPlanThreads + tid, stride = kPlanCluster * kPlanThreads;
+    __shared__ longlong2 s_totals[kPlanCluster];  // new tokens and pages asked for, by CTA
+    __shared__ int2 s_outcome[kPlanCluster];      // pages taken up to there and requests refused, by CTA
+    __shared__ int s_taken;
+    const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool lead = blockIdx.x < kPlanCluster;  // the cluster that writes the lengths and counts
+    const int all = blockIdx.x * kPlanThreads + tid, stride = gridDim.x * kPlanThreads;
     const int page = static_cast<int>(p.page.d);
     const long long free_count = min(max(*p.free_count, 0), p.free_capacity);
     long long tokens = 0, asked = 0;  // of the rounds before
-    long long taken = 0;              // this thread's largest end of a served request's pages
-    int refused = 0;
+    int taken = 0, refused = 0;       // rank 0, thread 0
 
-    for (int base = 0; base < p.requests; base += kPlanRound) {
+    // An empty step is one round too: the barriers stand between reading free_count and writing left.
+    for (int base = 0; base == 0 || base < p.requests; base += kPlanRound) {
         const int n = min(kPlanRound, p.requests - base);
-        int held[kPlanPer], added[kPlanPer], have[kPlanPer], need[kPlanPer];
-        bool fits[kPlanPer];
-        long long a = 0, b = 0;
+        const int each = (n + kPlanCluster - 1) / kPlanCluster, bits = n > 1 ? 32 - __clz(n - 1) : 0;
+        const int r = rank * each + tid;
+        const bool mine = tid < each && r < n;
+        const int held = mine ? p.held[base + r] : 0, added = mine ? p.added[base + r] : 0;
+        const uint32_t h = max(held, 0), m = max(added, 0), end = h + m;  // < 2^32
+        const int have = static_cast<int>(p.page.div(h) + (h != p.page.div(h) * p.page.d));
+        const uint32_t want = end / p.page.d + (end % p.page.d != 0);
+        const bool fits = held >= 0 && added >= 0 && want <= static_cast<uint32_t>(p.width);
+        const int need = fits ? static_cast<int>(want) - have : 0;
+        // Exclusive prefixes (a, b) over the CTA.
+        long long a = m, b = need;
 #pragma unroll
-        for (int i = 0; i < kPlanPer; ++i) {
-            const int r = tid * kPlanPer + i;
-            held[i] = r < n ? p.held[base + r] : 0;
-            added[i] = r < n ? p.added[base + r] : 0;
-            const uint32_t h = max(held[i], 0), m = max(added[i], 0);
-            have[i] = static_cast<int>(p.page.div(h) + (h % p.page.d != 0));
-            const uint32_t last = h + m;  // < 2^32
-            const uint32_t want = last / p.page.d + (last % p.page.d != 0);
-            fits[i] = held[i] >= 0 && added[i] >= 0 && want <= static_cast<uint32_t>(p.width);
-            need[i] = fits[i] ? static_cast<int>(want) - have[i] : 0;
-            a += m;
-            b += need[i];
-        }
-        long long round_tokens, round_asked;
-        block_scan2(a, b, round_tokens, round_asked, warp_sums);
-        cluster_sync_all();  // every CTA has read this round's lengths (and, in round 0, free_count)
-#pragma unroll
-        for (int i = 0; i < kPlanPer; ++i) {
-            const int r = tid * kPlanPer + i;
-            if (r < n) {
-                const bool served = fits[i] && (need[i] == 0 || asked + b + need[i] <= free_count);
-                s_start[r] = static_cast<int>(min(a, 0x7FFFFFFFLL));
-                s_first[r] = static_cast<int>(min(b, 0x7FFFFFFFLL));
-                s_held[r] = max(held[i], 0);
-                s_have[r] = served ? have[i] : -1;
-                if (served && need[i] > 0) taken = max(taken, asked + b + need[i]);
-                refused += !served;
-                if (rank == r % kPlanCluster) {
-                    p.seq_lens[base + r] = served ? held[i] + added[i] : held[i];
-                    if (p.starts != nullptr)
-                        p.starts[base + r] = static_cast<int>(min(tokens + a, p.slot_capacity));
-                }
-                a += max(added[i], 0);
-                b += need[i];
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long xa = __shfl_up_sync(~0u, a, o), xb = __shfl_up_sync(~0u, b, o);
+            if (lane >= o) {
+                a += xa;
+                b += xb;
             }
         }
+        if (lane == 31) {
+            warp_sums[warp][0] = a;
+            warp_sums[warp][1] = b;
+        }
+        a -= m;
+        b -= need;
+        if (tid == 0) s_taken = 0;
         __syncthreads();
+        {
+            // Every warp sums the warps before it, and the CTA's total.
+            long long wa = warp_sums[lane][0], wb = warp_sums[lane][1];
+            long long la = lane < warp ? wa : 0, lb = lane < warp ? wb : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                wa += __shfl_xor_sync(~0u, wa, o);
+                wb += __shfl_xor_sync(~0u, wb, o);
+                la += __shfl_xor_sync(~0u, la, o);
+                lb += __shfl_xor_sync(~0u, lb, o);
+            }
+            a += la;
+            b += lb;
+            if (tid < kPlanCluster) cluster_store(cluster_address(smem_u32(&s_totals[rank]), tid), wa, wb);
+        }
+        cluster_sync_all();  // totals; every CTA has read its lengths (and, in round 0, free_count)
+        long long round_tokens = 0, round_asked = 0;
+#pragma unroll
+        for (int c = 0; c < kPlanCluster; ++c) {
+            const longlong2 x = s_totals[c];
+            if (c < rank) {
+                a += x.x;
+                b += x.y;
+            }
+            round_tokens += x.x;
+            round_asked += x.y;
+        }
+        const bool served = fits && (need == 0 || asked + b + need <= free_count);
+        const int out = __syncthreads_count(mine && !served);
+        const int end_page = mine && served && need > 0 ? static_cast<int>(asked + b + need) : 0;  // <= free_count
+        const int most = __reduce_max_sync(~0u, end_page);
+        if (lane == 0 && most > 0) atomicMax(&s_taken, most);
+        if (mine) {
+            const int4 x = make_int4(static_cast<int>(min(a, 0x7FFFFFFFLL)), static_cast<int>(min(b, 0x7FFFFFFFLL)),
+                                     static_cast<int>(h), served ? have : -1);
+#pragma unroll
+            for (int c = 0; c < kPlanCluster; ++c) cluster_store(cluster_address(smem_u32(s_req + r), c), x);
+            if (lead) {
+                p.seq_lens[base + r] = served ? held + added : held;
+                if (p.starts != nullptr) p.starts[base + r] = static_cast<int>(min(tokens + a, p.slot_capacity));
+            }
+        }
+        __syncthreads();  // s_taken
+        if (tid == 0) cluster_store(cluster_address(smem_u32(&s_outcome[rank]), 0), s_taken, out);
+        cluster_sync_all();  // the prefixes and outcomes
+        if (rank == 0 && tid == 0) {
+            for (int c = 0; c < kPlanCluster; ++c) {
+                taken = max(taken, s_outcome[c].x);
+                refused += s_outcome[c].y;
+            }
+        }
         // Slots and positions of this round's tokens.
+        const int *const free_top = p.free_pages + (free_count - 1 - asked);  // read only where a page is left
         const long long room = min(round_tokens, max(0LL, p.slot_capacity - tokens));
         for (long long t = all; t < room; t += stride) {
-            const int r = last_at_most(s_start, n, static_cast<int>(t));
-            const uint32_t position = static_cast<uint32_t>(s_held[r]) + static_cast<uint32_t>(t - s_start[r]);
-            const int have_r = s_have[r];
+            const int at = last_at_most(&s_req->x, n, bits, static_cast<int>(t));
+            const int4 req = s_req[at];
+            const uint32_t position = static_cast<uint32_t>(req.z) + static_cast<uint32_t>(static_cast<int>(t) - req.x);
             long long slot = -1;
-            if (have_r >= 0) {
+            if (req.w >= 0) {
                 const int col = static_cast<int>(p.page.div(position));
-                const int id = col < have_r
-                                   ? p.table[(base + r) * p.table_stride + col]
-                                   : p.free_pages[free_count - 1 - (asked + s_first[r] + (col - have_r))];
+                const int id = col < req.w ? p.table[(base + at) * p.table_stride + col]
+                                           : free_top[-(req.y + (col - req.w))];
                 if (id >= 0) slot = static_cast<long long>(id) * page + (position - static_cast<uint32_t>(col) * page);
             }
             p.slots[tokens + t] = slot;
@@ -192,45 +213,25 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
         // Table entries of the pages taken (those asked for past the stack are nobody's).
         const long long pages = min(round_asked, free_count - asked);
         for (long long i = all; i < pages; i += stride) {
-            const int r = last_at_most(s_first, n, static_cast<int>(i));
-            if (s_have[r] >= 0)
-                p.table[(base + r) * p.table_stride + s_have[r] + (static_cast<int>(i) - s_first[r])] =
-                    p.free_pages[free_count - 1 - (asked + i)];
+            const int x = static_cast<int>(i), at = last_at_most(&s_req->y, n, bits, x);
+            const int4 req = s_req[at];
+            if (req.w >= 0) p.table[(base + at) * p.table_stride + req.w + (x - req.y)] = free_top[-x];
         }
         tokens += round_tokens;
         asked += round_asked;
-        __syncthreads();
     }
-    if (p.requests == 0) cluster_sync_all();  // free_count read by all before left is written
     for (long long t = tokens + all; t < p.slot_capacity; t += stride) {
         p.slots[t] = -1;
         if (p.positions != nullptr) p.positions[t] = 0;
     }
-    if (rank == 0) {
-        long long most = taken, sum = refused;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            most = max(most, __shfl_xor_sync(~0u, most, o));
-            sum += __shfl_xor_sync(~0u, sum, o);
-        }
-        if ((tid & 31) == 0) {
-            warp_sums[tid >> 5][0] = most;
-            warp_sums[tid >> 5][1] = sum;
-        }
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 1; w < kPlanThreads / 32; ++w) {
-                most = max(most, warp_sums[w][0]);
-                sum += warp_sums[w][1];
-            }
-            *p.left = static_cast<int>(free_count - most);
-            if (p.starts != nullptr) p.starts[p.requests] = static_cast<int>(min(tokens, p.slot_capacity));
-            if (p.status != nullptr) {
-                p.status[0] = static_cast<int>(min(tokens, 0x7FFFFFFFLL));
-                p.status[1] = static_cast<int>(most);
-                p.status[2] = static_cast<int>(sum);
-                p.status[3] = static_cast<int>(min(max(0LL, tokens - p.slot_capacity), 0x7FFFFFFFLL));
-            }
+    if (lead && rank == 0 && tid == 0) {
+        *p.left = static_cast<int>(free_count) - taken;
+        if (p.starts != nullptr) p.starts[p.requests] = static_cast<int>(min(tokens, p.slot_capacity));
+        if (p.status != nullptr) {
+            p.status[0] = static_cast<int>(min(tokens, 0x7FFFFFFFLL));
+            p.status[1] = taken;
+            p.status[2] = refused;
+            p.status[3] = static_cast<int>(min(max(0LL, tokens - p.slot_capacity), 0x7FFFFFFFLL));
         }
     }
 }
@@ -245,14 +246,15 @@ struct AppendParams {
     long long k_tok, k_head, v_tok, v_head;                // bytes
     long long ck_page, ck_tok, ck_head, cv_page, cv_tok, cv_head;  // bytes
     long long tokens, num_slots;
-    int chunks;        // 8-element pieces of a token's row of one of K or V: kv_heads * head_dim / 8
-    int head_chunks;   // head_dim / 8
+    int pieces;        // pieces (kAppendPiece elements) of a token's row of one of K or V: kv_heads * head_pieces
+    int head_pieces;   // head_dim / kAppendPiece
     int group;         // tokens per block
     bool vec;          // k, v and their strides are 16-byte multiples
     uint32_t page_size;
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendPiece = 16;  // elements of K, and as many of V, that a thread moves at once
 
 __device__ __forceinline__ uint4 load8(const char *p, bool vec) {
     if (vec) return __ldg(reinterpret_cast<const uint4 *>(p));
@@ -274,47 +276,70 @@ __device__ __forceinline__ float2 unpack16(uint32_t w) {
     }
 }
 
-// Two e4m3 values of (a / s, b / s), round to nearest even, saturating.
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b, float s) {
-    const float2 x = make_float2(__fdiv_rn(a, s), __fdiv_rn(b, s));
-    return __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
-}
-
-template <int kIn, bool kQuant>
-__device__ __forceinline__ void append_piece(char *dst, const uint4 &x, float s) {
-    if constexpr (kQuant) {
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t q[4];
+// e4m3 of eight elements x / s, round to nearest even, saturating.  `below` and
+// `above` are 1 / s less and more 2^-21 of it, so that x / s, rounded to f32 or
+// not, lies between the two products; where both round to the same e4m3, as
+// they do for all but one element in 10^5, so does it.  Only else (or where
+// 1 / s leaves the normal range, below = above = 0) is the quotient computed.
+// Dividing always took 10.1 us instead of 7.7 us for 10007 rows of 4 x 128 bf16.
+template <int kIn>
+__device__ __forceinline__ uint2 quantise8(const uint4 &x, float s, float below, float above) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t q[4], differ = below == 0.0f ? 1u : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack16<kIn == kBF16>(w[i]);
+        q[i] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * below, f.y * below), __NV_SATFINITE, __NV_E4M3);
+        differ |= q[i] ^ __nv_cvt_float2_to_fp8x2(make_float2(f.x * above, f.y * above), __NV_SATFINITE, __NV_E4M3);
+    }
+    if (differ != 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = unpack16<kIn == kBF16>(w[i]);
-            q[i] = e4m3x2(f.x, f.y, s);
+            q[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s)), __NV_SATFINITE,
+                                            __NV_E4M3);
         }
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+    }
+    return make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+}
+
+template <int kIn, bool kQuant>
+__device__ __forceinline__ void append_piece(char *dst, const uint4 &x, const uint4 &y, float s) {
+    if constexpr (kQuant) {
+        const float inverse = 1.0f / s, size = fabsf(inverse);
+        const float r = size >= 1e-37f && size <= 1e37f ? inverse : 0.0f;
+        const float below = r * (1.0f - 0x1p-21f), above = r * (1.0f + 0x1p-21f);
+        const uint2 a = quantise8<kIn>(x, s, below, above), b = quantise8<kIn>(y, s, below, above);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(a.x, a.y, b.x, b.y);
     } else {
-        *reinterpret_cast<uint4 *>(dst) = x;
+        reinterpret_cast<uint4 *>(dst)[0] = x;
+        reinterpret_cast<uint4 *>(dst)[1] = y;
     }
 }
 
-// A thread moves 8 elements of a K row and the 8 at the same place of the V
-// row.  kIn is the rows' type (read only where they are quantised).
+// A thread moves 16 elements of a K row and the 16 at the same place of the V
+// row: four 16-byte loads in flight.  kIn is the rows' type (read only where
+// they are quantised).
 template <int kIn, bool kQuant>
 __global__ void __launch_bounds__(kAppendThreads) paged_append(const AppendParams p) {
     const long long t0 = static_cast<long long>(blockIdx.x) * p.group;
-    const int count = static_cast<int>(min(static_cast<long long>(p.group), p.tokens - t0)) * p.chunks;
+    const int count = static_cast<int>(min(static_cast<long long>(p.group), p.tokens - t0)) * p.pieces;
     for (int i = threadIdx.x; i < count; i += kAppendThreads) {
-        const int local = i / p.chunks, c = i - local * p.chunks;
-        const int h = c / p.head_chunks, piece = c - h * p.head_chunks;
-        const long long t = t0 + local, slot = p.slots[t];
+        const int local = i / p.pieces, c = i - local * p.pieces;
+        const int h = c / p.head_pieces, piece = c - h * p.head_pieces;
+        const long long t = t0 + local;
+        const char *const k = p.k + t * p.k_tok + h * p.k_head + piece * (2 * kAppendPiece);
+        const char *const v = p.v + t * p.v_tok + h * p.v_head + piece * (2 * kAppendPiece);
+        const long long slot = p.slots[t];
+        const uint4 k0 = load8(k, p.vec), k1 = load8(k + 16, p.vec);
+        const uint4 v0 = load8(v, p.vec), v1 = load8(v + 16, p.vec);
         if (slot < 0 || slot >= p.num_slots) continue;
-        const uint4 k = load8(p.k + t * p.k_tok + h * p.k_head + piece * 16, p.vec);
-        const uint4 v = load8(p.v + t * p.v_tok + h * p.v_head + piece * 16, p.vec);
         const long long page = slot / p.page_size, row = slot - page * p.page_size;
-        const int bytes = kQuant ? 8 : 16;
+        const int at = piece * kAppendPiece * (kQuant ? 1 : 2);
         const float ks = kQuant && p.k_scale != nullptr ? p.k_scale[h] : 1.0f;
         const float vs = kQuant && p.v_scale != nullptr ? p.v_scale[h] : 1.0f;
-        append_piece<kIn, kQuant>(p.ck + page * p.ck_page + row * p.ck_tok + h * p.ck_head + piece * bytes, k, ks);
-        append_piece<kIn, kQuant>(p.cv + page * p.cv_page + row * p.cv_tok + h * p.cv_head + piece * bytes, v, vs);
+        append_piece<kIn, kQuant>(p.ck + page * p.ck_page + row * p.ck_tok + h * p.ck_head + at, k0, k1, ks);
+        append_piece<kIn, kQuant>(p.cv + page * p.cv_page + row * p.cv_tok + h * p.cv_head + at, v0, v1, vs);
     }
 }
 
@@ -340,11 +365,6 @@ struct DecodeParams {
     float scale_log2;
     int records_by_item;
     int q_bf16, o_dtype, q_vec, o_vec, p_parts;
-};
-
-template <bool kValue>
-struct Flag {
-    static constexpr bool value = kValue;
 };
 
 constexpr int kWarps = 4;
@@ -1035,9 +1055,9 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                 }
             };
             if (groups == (1u << KS) - 1)
-                products(Flag<true>());
+                products(Constant<true>());
             else
-                products(Flag<false>());
+                products(Constant<false>());
         }
 
         const bool item_done = at.tile + 1 == at.tiles;
