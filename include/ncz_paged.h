@@ -133,7 +133,7 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * window has passed them): their keys are left out.  A row without keys gives
  * o = 0 and lse = -infinity.  Nothing in an absent page or behind len affects
  * the result.  Scores, softmax and sums are f32; P is kept in two 16-bit parts
- * (three for bf16 K/V with f32 o), so o has f32 accuracy before its rounding.
+ * (three for bf16 K/V with f32 o).
  *
  * q is f16 or bf16 (the cache's type; either for e4m3); o is f32, f16 or bf16;
  * lse may be NULL, else f32 [batch][q_heads].  q and o may have any strides
@@ -168,6 +168,20 @@ typedef struct ncz_paged_decode_desc {
 } ncz_paged_decode_desc;
 
 int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *desc);
+
+/* Synchronises `device` (-1 = current), then reads and clears the bounded-wait
+ * status word of its decode kernels: NCZ_SUCCESS, or NCZ_ERROR_DEVICE_TIMEOUT
+ * when a wait inside a kernel ran past the wait limit since the last call (that
+ * kernel then stopped cleanly; its o and lse are incomplete). */
+int ncz_paged_sync_status(int device);
+
+/* Test hooks (failure detection without a GPU fault), device -1 = current.
+ * ncz_paged_test_set_wait_limit: bound of every in-kernel wait in SM cycles (0
+ * restores the default, about 2 s).  ncz_paged_test_drop_scores: while enabled,
+ * the first CTA of a launch for 17 or more query heads per K/V head never
+ * announces its first scores, so a wait runs out. */
+int ncz_paged_test_set_wait_limit(int device, uint64_t cycles);
+int ncz_paged_test_drop_scores(int device, int enable);
 
 /* Bytes of workspace for ncz_paged_decode on `device` (-1 = current). */
 int ncz_paged_decode_workspace(const ncz_paged_cache *cache, size_t q_heads, int device, size_t *bytes);

@@ -8,7 +8,7 @@
 #include "driver.cuh"
 #include "ncz_flash.h"
 #include "ncz_paged.h"
-#include "paged_sm100.cuh"
+#include "paged_wide_sm100.cuh"
 #include "status.cuh"
 
 namespace {
@@ -32,6 +32,7 @@ struct Kernel {
     int smem;
     int ctas;  // decode: CTAs per SM
     int tile;  // decode: keys a CTA takes per step
+    int threads;
     bool ready[kMaxDevices];
 };
 
@@ -41,12 +42,12 @@ const void *decode_fn() {
 }
 #define NCZ_DECODE(D, KV, KVNAME, NT) \
     {decode_fn<D, KV, NT>(), "paged_decode<" #D "," KVNAME "," #NT ">", nczp::Decode<D, KV, NT>::kSmem, \
-     nczp::Decode<D, KV, NT>::kCtas, nczp::Decode<D, KV, NT>::kTile, {}}
+     nczp::Decode<D, KV, NT>::kCtas, nczp::Decode<D, KV, NT>::kTile, nczp::kDecodeThreads, {}}
 #define NCZ_DECODE_NT(D, KV, KVNAME) \
     {NCZ_DECODE(D, KV, KVNAME, 1), NCZ_DECODE(D, KV, KVNAME, 2), NCZ_DECODE(D, KV, KVNAME, 4)}
 #define NCZ_DECODE_D(KV, KVNAME, FIRST) \
     {FIRST, NCZ_DECODE_NT(32, KV, KVNAME), NCZ_DECODE_NT(64, KV, KVNAME), NCZ_DECODE_NT(128, KV, KVNAME)}
-#define NCZ_NONE {{nullptr, nullptr, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, {}}}
+#define NCZ_NONE {{nullptr, nullptr, 0, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, 0, {}}, {nullptr, nullptr, 0, 0, 0, 0, {}}}
 
 // [cache type - 1][log2(head_dim) - 4][log2(query heads per item / 8)]
 Kernel g_decode[3][4][3] = {
@@ -54,18 +55,34 @@ Kernel g_decode[3][4][3] = {
     NCZ_DECODE_D(nczp::kBF16, "bf16", NCZ_DECODE_NT(16, nczp::kBF16, "bf16")),
     NCZ_DECODE_D(nczp::kE4M3, "e4m3", NCZ_NONE),
 };
+template <int D, bool kBf16, int kQRows>
+const void *wide_fn() {
+    return reinterpret_cast<const void *>(nczp::paged_decode_wide<nczp::Wide<D, kBf16, kQRows>>);
+}
+#define NCZ_WIDE(D, BF16, NAME, ROWS) \
+    {wide_fn<D, BF16, ROWS>(), "paged_decode_wide<" #D "," NAME "," #ROWS ">", nczp::Wide<D, BF16, ROWS>::kSmem, 1, \
+     nczp::kWideTile, nczp::Wide<D, BF16, ROWS>::kThreads, {}}
+
+#define NCZ_WIDE_ROWS(D, BF16, NAME) \
+    {NCZ_WIDE(D, BF16, NAME, 32), NCZ_WIDE(D, BF16, NAME, 64), NCZ_WIDE(D, BF16, NAME, 128)}
+
+// [bf16][head_dim 64, 128][32, 64, 128 query heads]
+Kernel g_wide[2][2][3] = {
+    {NCZ_WIDE_ROWS(64, false, "f16"), NCZ_WIDE_ROWS(128, false, "f16")},
+    {NCZ_WIDE_ROWS(64, true, "bf16"), NCZ_WIDE_ROWS(128, true, "bf16")},
+};
 Kernel g_join[4] = {
-    {reinterpret_cast<const void *>(nczp::paged_join<16>), "paged_join<16>", 0, 0, 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<32>), "paged_join<32>", 0, 0, 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<64>), "paged_join<64>", 0, 0, 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_join<128>), "paged_join<128>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<16>), "paged_join<16>", 0, 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<32>), "paged_join<32>", 0, 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<64>), "paged_join<64>", 0, 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_join<128>), "paged_join<128>", 0, 0, 0, 0, {}},
 };
 Kernel g_append[3] = {
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, false>), "paged_append<copy>", 0, 0, 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, true>), "paged_append<f16,e4m3>", 0, 0, 0, {}},
-    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kBF16, true>), "paged_append<bf16,e4m3>", 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, false>), "paged_append<copy>", 0, 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kF16, true>), "paged_append<f16,e4m3>", 0, 0, 0, 0, {}},
+    {reinterpret_cast<const void *>(nczp::paged_append<nczp::kBF16, true>), "paged_append<bf16,e4m3>", 0, 0, 0, 0, {}},
 };
-Kernel g_plan = {reinterpret_cast<const void *>(nczp::paged_plan), "paged_plan", nczp::kPlanSmem, 0, 0, {}};
+Kernel g_plan = {reinterpret_cast<const void *>(nczp::paged_plan), "paged_plan", nczp::kPlanSmem, 0, 0, 0, {}};
 
 template <class Fn>
 void each_kernel(Fn fn) {
@@ -73,6 +90,9 @@ void each_kernel(Fn fn) {
         for (auto &by_rows : by_dim)
             for (Kernel &k : by_rows)
                 if (k.fn != nullptr) fn(k);
+    for (auto &by_dim : g_wide)
+        for (auto &by_rows : by_dim)
+            for (Kernel &k : by_rows) fn(k);
     for (Kernel &k : g_join) fn(k);
     for (Kernel &k : g_append) fn(k);
     fn(g_plan);
@@ -181,8 +201,43 @@ int rows_index(size_t group) { return group <= 8 ? 0 : group <= 16 ? 1 : 2; }
 
 int dim_index(size_t d) { return d == 16 ? 0 : d == 32 ? 1 : d == 64 ? 2 : 3; }
 
-Kernel &decode_kernel(const ncz_paged_cache &c, size_t group) {
-    return g_decode[c.dtype - 1][dim_index(c.head_dim)][rows_index(group)];
+// The kernel of a call and the query heads of its items.
+struct Choice {
+    Kernel *kernel;
+    int rows;
+};
+
+Choice narrow_choice(const ncz_paged_cache &c, size_t group) {
+    const int i = rows_index(group);
+    return {&g_decode[c.dtype - 1][dim_index(c.head_dim)][i], 8 << i};
+}
+
+// Whether the tcgen05 kernel exists for a cache and pays for a group of query
+// heads: from 17 on (batch 16, 4 K/V heads, 8192 keys, head_dim 64: 16 query heads
+// 38.7 us with the warp MMAs and 40.1 us with it, 24: 55.8 and 40.6), at
+// head_dim 128 from 9 on (12: 59.6 and 56.3, 32: 86.5 and 58.5; 8: 50.2 and 55.6).
+bool has_wide(const ncz_paged_cache &c, size_t group) {
+    return c.dtype != NCZ_DTYPE_E4M3 && c.head_dim >= 64 && group >= (c.head_dim == 128 ? 9 : 17);
+}
+
+Choice wide_choice(const ncz_paged_cache &c, size_t group) {
+    const int i = group <= 32 ? 0 : group <= 64 ? 1 : 2;
+    return {&g_wide[c.dtype == NCZ_DTYPE_BF16][c.head_dim == 128][i], 32 << i};
+}
+
+// The kernel of a call over up to `keys` keys a request.  f32 outputs stay with
+// the warp MMAs: those sums are added in f32 every step, while tensor memory
+// accumulates (and cuts off) over a row's whole length.  So do small launches:
+// the tcgen05 kernel takes 128 keys a step and starts and ends slower (32 query
+// heads of 8 K/V heads, head_dim 128: one request of 2000 keys, 128 steps in all,
+// 14.4 us with the warp MMAs and 15.0 us with it, of 8000 keys 23.6 and 19.3;
+// 64 requests of 300 keys, 3 steps each, 46.1 and 52.4, of 1000 keys 92.0 and 73.2).
+Choice choose(const ncz_paged_cache &c, size_t group, int o_dtype, size_t batch, size_t keys, int sms) {
+    const Choice narrow = narrow_choice(c, group);
+    if (!has_wide(c, group) || o_dtype == NCZ_DTYPE_F32) return narrow;
+    const Choice wide = wide_choice(c, group);
+    const size_t each = (keys + nczp::kWideTile - 1) / nczp::kWideTile, blocks = (group + wide.rows - 1) / wide.rows;
+    return each >= 4 && batch * c.kv_heads * blocks * each >= 2 * static_cast<size_t>(sms) ? wide : narrow;
 }
 
 // CTAs of a launch at most: what is resident at once.
@@ -310,9 +365,14 @@ int ncz_paged_decode_workspace(const ncz_paged_cache *cache, size_t q_heads, int
     st = check_heads(*cache, q_heads);
     if (st != NCZ_SUCCESS) return st;
     const size_t group = q_heads / cache->kv_heads;
-    const Kernel &k = decode_kernel(*cache, group);
     return on_device(device, [&](int dev) {
-        *bytes = workspace_need(k, cache->head_dim, 8 << rows_index(group), device_sms(dev));
+        // For any batch and output type: the larger of the kernels that may be taken.
+        const Choice narrow = narrow_choice(*cache, group);
+        *bytes = workspace_need(*narrow.kernel, cache->head_dim, narrow.rows, device_sms(dev));
+        if (has_wide(*cache, group)) {
+            const Choice wide = wide_choice(*cache, group);
+            *bytes = std::max(*bytes, workspace_need(*wide.kernel, cache->head_dim, wide.rows, device_sms(dev)));
+        }
         return NCZ_SUCCESS;
     });
 }
@@ -342,10 +402,6 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     const size_t o_size = static_cast<size_t>(element_size(d.o_dtype));
     if (!aligned(d.q, 2) || !aligned(d.o, o_size)) return NCZ_ERROR_MISALIGNED;
     const size_t group = d.q_heads / c.kv_heads;
-    const int rows = 8 << rows_index(group);
-    const size_t blocks = (group + rows - 1) / rows;
-    Kernel &k = decode_kernel(c, group);
-
     nczp::DecodeParams p{};
     p.q = static_cast<const char *>(d.q);
     p.k = static_cast<const char *>(c.k);
@@ -370,8 +426,6 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     p.table_stride = static_cast<long long>(d.table_stride);
     p.batch = static_cast<int>(d.batch);
     p.group = static_cast<int>(group);
-    p.blocks = static_cast<int>(blocks);
-    p.head_blocks = static_cast<int>(c.kv_heads * blocks);
     p.width_keys = static_cast<int>(d.table_width * c.page_size);
     p.window = static_cast<int>(std::min(d.window, kMaxInt));
     p.num_pages = static_cast<int>(c.num_pages);
@@ -385,13 +439,20 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     p.o_vec = aligned(d.o, 4 * o_size) && d.o_batch_stride % 4 == 0 && d.o_head_stride % 4 == 0;
     p.p_parts = c.dtype == NCZ_DTYPE_BF16 && d.o_dtype == NCZ_DTYPE_F32 ? 3 : 2;
 
+    // Keys of a request at most: the lengths are on the device, the table's width bounds them.
+    const size_t keys = d.window > 0 ? std::min(d.window, static_cast<size_t>(p.width_keys)) : p.width_keys;
+
     return on_device(d.device, [&](int dev) {
         const int sms = device_sms(dev);
+        const Choice choice = choose(c, group, d.o_dtype, d.batch, keys, sms);
+        Kernel &k = *choice.kernel;
+        const int rows = choice.rows;
+        const size_t blocks = (group + rows - 1) / rows;
+        p.blocks = static_cast<int>(blocks);
+        p.head_blocks = static_cast<int>(c.kv_heads * blocks);
         if (d.workspace == nullptr || d.workspace_bytes < workspace_need(k, c.head_dim, rows, sms))
             return static_cast<int>(NCZ_ERROR_OUT_OF_MEMORY);
         if (!aligned(d.workspace, 16)) return static_cast<int>(NCZ_ERROR_MISALIGNED);
-        // Tiles at most: the lengths are on the device, the table's width bounds them.
-        const size_t keys = d.window > 0 ? std::min(d.window, static_cast<size_t>(p.width_keys)) : p.width_keys;
         const size_t tile = static_cast<size_t>(k.tile);
         const size_t most = std::max<size_t>(1, (keys + (d.window > 0 ? 15 : 0) + tile - 1) / tile);
         const size_t items = d.batch * static_cast<size_t>(p.head_blocks);
@@ -406,7 +467,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         p.part_o = reinterpret_cast<float *>(ws + records_bytes(ctas));
         p.part_ml = reinterpret_cast<float2 *>(p.part_o + 2 * static_cast<size_t>(ctas) * rows * c.head_dim);
         void *args[1] = {&p};
-        int s = launch(k, grid, nczp::kDecodeThreads, dev, d.stream, args);
+        int s = launch(k, grid, k.threads, dev, d.stream, args);
         // Rows of one tile are whole in one CTA: nothing to join.
         if (s != NCZ_SUCCESS || most == 1) return s;
         // Quads (four elements) per join block: as few as keep the grid within
@@ -422,6 +483,35 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         void *join_args[4] = {&p, &join_rows, &quads, &per_record};
         return launch(g_join[dim_index(c.head_dim)], records * per_record, nczp::kJoinThreads, dev, d.stream,
                       join_args);
+    });
+}
+
+int ncz_paged_sync_status(int device) {
+    return on_device(device, [](int) {
+        uint32_t word = 0;
+        const void *sym = static_cast<const void *>(&nczp::g_paged_status);
+        int e = drv().device_synchronize();
+        if (e == cudaSuccess) e = drv().symbol_read(&word, sym, sizeof(word));
+        if (e == cudaSuccess && word != 0) {
+            const uint32_t zero = 0;
+            e = drv().symbol_write(sym, &zero, sizeof(zero));
+        }
+        if (e != cudaSuccess) return map_cuda_error(e);
+        return static_cast<int>(word != 0 ? NCZ_ERROR_DEVICE_TIMEOUT : NCZ_SUCCESS);
+    });
+}
+
+int ncz_paged_test_set_wait_limit(int device, uint64_t cycles) {
+    const unsigned long long v = cycles != 0 ? cycles : nczp::kPagedWaitLimit;
+    return on_device(device, [&](int) {
+        return map_cuda_error(drv().symbol_write(static_cast<const void *>(&nczp::g_paged_wait_limit), &v, sizeof(v)));
+    });
+}
+
+int ncz_paged_test_drop_scores(int device, int enable) {
+    const int v = enable != 0;
+    return on_device(device, [&](int) {
+        return map_cuda_error(drv().symbol_write(static_cast<const void *>(&nczp::g_paged_test_drop), &v, sizeof(v)));
     });
 }
 

@@ -64,6 +64,9 @@ _SIGNATURES = {
     "ncz_paged_plan": (ctypes.c_int, [ctypes.POINTER(_Plan)]),
     "ncz_paged_append": (ctypes.c_int, [ctypes.POINTER(_Cache), ctypes.POINTER(_Append)]),
     "ncz_paged_decode": (ctypes.c_int, [ctypes.POINTER(_Cache), ctypes.POINTER(_Decode)]),
+    "ncz_paged_sync_status": (ctypes.c_int, [ctypes.c_int]),
+    "ncz_paged_test_set_wait_limit": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
+    "ncz_paged_test_drop_scores": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
     "ncz_paged_decode_workspace": (ctypes.c_int, [ctypes.POINTER(_Cache), _SZ, ctypes.c_int, ctypes.POINTER(_SZ)]),
 }
 _bound: Optional[ctypes.CDLL] = None
@@ -280,6 +283,14 @@ def _call_workspace(cache: Cache, heads: int, stream, handle: int):
         return decode_workspace(cache, heads)
     with _torch.cuda.stream(_torch.cuda.ExternalStream(handle, device=cache.device)):
         return decode_workspace(cache, heads)
+
+
+def sync_status(device: Optional[int] = None) -> int:
+    """Synchronises `device` and raises FlashError(DeviceTimeout) when a bounded
+    wait of a decode kernel ran out since the last call."""
+    st = lib().ncz_paged_sync_status(-1 if device is None else device)
+    flash._check(st, "paged.sync_status")
+    return st
 
 
 def decode_flops(keys: int, q_heads: int, head_dim: int) -> int:

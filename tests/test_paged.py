@@ -155,6 +155,37 @@ def test_decode_kernels_by_type_and_group(ncz, fake):
                 assert labels(ncz, fake.launches) == [f"paged_decode<{dim},{name},{rows}>", f"paged_join<{dim}>"]
 
 
+def test_decode_kernel_for_many_heads_per_kv_head(ncz, fake):
+    """The tcgen05 kernel: 16-bit caches, head_dim 64 or 128, enough query heads and
+    steps of 128 keys, 16-bit outputs; one CTA per SM."""
+    def label(dim, group, dtype=BF16, o_dtype=BF16, batch=64, width=64, kv=1):
+        fake.launches.clear()
+        q_dtype = BF16 if dtype == E4M3 else dtype
+        d = decode_desc(ncz, q_heads=kv * group, dim=dim, q_dtype=q_dtype, o_dtype=o_dtype, batch=batch, width=width)
+        assert run(ncz, "ncz_paged_decode", cache(ncz, kv=kv, dim=dim, dtype=dtype), d) == "Success"
+        return labels(ncz, fake.launches)[0]
+
+    assert label(64, 17) == "paged_decode_wide<64,bf16,32>" and fake.launches[0].grid == 148
+    assert label(64, 33, F16, F16) == "paged_decode_wide<64,f16,64>"
+    assert label(128, 65) == "paged_decode_wide<128,bf16,128>" and label(128, 300) == "paged_decode_wide<128,bf16,128>"
+    assert label(128, 9) == "paged_decode_wide<128,bf16,32>" and label(64, 16) == "paged_decode<64,bf16,2>"
+    assert label(128, 8) == "paged_decode<128,bf16,1>"
+    for other in (label(32, 32), label(128, 32, E4M3), label(128, 32, o_dtype=F32), label(128, 32, batch=30),
+                  label(128, 32, width=24)):
+        assert other.startswith("paged_decode<")
+    assert label(128, 32, batch=4, kv=8, width=96).startswith("paged_decode_wide<")
+
+
+def test_status_word_and_hooks(ncz, fake):
+    lib = ncz.paged.lib()
+    assert ncz.paged.sync_status(3) == 0
+    fake.symbol_words[3] = 0x81000005
+    assert status(ncz, lib.ncz_paged_sync_status(3)) == "DeviceTimeout"
+    assert ncz.paged.sync_status(3) == 0 and fake.current() == 0
+    assert lib.ncz_paged_test_set_wait_limit(2, 5) == 0 and lib.ncz_paged_test_drop_scores(2, 1) == 0
+    assert [(dev, len(x)) for dev, x in fake.symbol_writes[-2:]] == [(2, 8), (2, 4)]
+
+
 def test_decode_grid_and_join(ncz, fake):
     # 64 * 16 keys at most: the grid is what is resident at once, in whole sets of the 8 heads
     assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=100)) == "Success"

@@ -292,6 +292,102 @@ def test_decode_many_requests(ncz, batch):
     check_decode(ncz, pr, F32)
 
 
+# Many query heads per K/V head: the tcgen05 kernel takes launches of at least
+# two steps of 128 keys per SM (the table's width counts: a wide one is enough).
+WIDE_LENS = [0, 1, 127, 128, 129, 900, 1000, 256, 385, 640, 17, 5]
+
+
+def wide_problem(batch, group, kv, dim, page, lens, dtype, **kw):
+    pr = P.decode_problem(batch, kv * group, kv, dim, page, lens, dtype, width=-(-(148 * 2 * 128) // page), **kw)
+    return pr
+
+
+@pytest.mark.parametrize("dim,group", [(64, 17), (64, 32), (64, 33), (64, 64), (64, 100), (64, 130), (128, 9), (128, 32),
+                                       (128, 40), (128, 64), (128, 65), (128, 128)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_decode_many_heads_per_kv_head(ncz, dim, group, dtype):
+    pr = wide_problem(len(WIDE_LENS), group, 1, dim, 16, WIDE_LENS, dtype, seed=dim + group)
+    check_decode(ncz, pr, dtype)
+    assert ncz.paged.sync_status() == 0
+
+
+@pytest.mark.parametrize("dim,group,kv,page", [(64, 20, 3, 7), (128, 12, 2, 1), (128, 50, 2, 100), (64, 70, 1, 32)])
+@pytest.mark.parametrize("layout", ["plain", "heads_first", "padded"])
+def test_decode_many_heads_layouts_windows_and_items(ncz, dim, group, kv, page, layout):
+    """Several items a CTA (60 requests), parts that end and begin inside CTAs, a
+    window whose pages before it are gone, odd strides of q and o."""
+    rng = np.random.default_rng(dim + group)
+    lens = rng.integers(0, 900, 60).tolist()
+    pr = wide_problem(60, group, kv, dim, page, lens, BF16, seed=page)
+    check_decode(ncz, pr, BF16, layout=layout)
+    for b, n in enumerate(lens):
+        pr["table"][b, :max(0, n - 600) // page] = -1
+    wide = torch.zeros(60, kv * group, dim + 3, dtype=BF16, device="cuda")
+    wide[..., 1:dim + 1] = pr["q"].cuda()
+    hold = torch.full((60, kv * group, dim + 5), 9.0, dtype=F16, device="cuda")
+    o = hold[..., 3:dim + 3]
+    check_decode(ncz, pr, F16, window=600, layout=layout, q=wide[..., 1:dim + 1], o=o)
+    o.fill_(9.0)
+    assert bool((hold == 9).all())
+    assert ncz.paged.sync_status() == 0
+
+
+def test_decode_many_heads_large_scores_and_absent_pages(ncz):
+    pr = wide_problem(3, 24, 1, 128, 16, [1500, 2000, 900], F16, seed=8)
+    ramp = torch.linspace(0.01, 8, 2000)
+    for b in range(3):
+        for j in range(int(pr["lens"][b])):
+            p_, r = int(pr["table"][b, j // 16]), j % 16
+            pr["k"][p_, r] *= ramp[j] if b != 1 else ramp[1999 - j]
+    for scale in (1.0, -0.5, 0.0):
+        pr["scale"] = scale
+        check_decode(ncz, pr, F16)
+    pr["table"][0, 20:60] = -1
+    pr["table"][1, :] = 2**31 - 1
+    pr["table"][2, 0] = pr["k"].shape[0]
+    _, lse = check_decode(ncz, pr, F16)
+    assert bool(torch.isinf(lse[1]).all())
+
+
+def test_decode_many_heads_long_rows_match_few_heads(ncz):
+    """20000 keys a request: every head's output is that of the same head decoded
+    alone (warp MMAs), up to both roundings."""
+    group, dim, n, page = 32, 128, 20000, 32
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(2 * n // page, page, 1, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(2, group, dim, generator=g, device="cuda").bfloat16()
+    table = torch.randperm(2 * n // page, generator=g, device="cuda").int().view(2, -1)
+    lens = i32([n, n - 77])
+    cache = ncz.paged.Cache(k, v)
+    o, one = torch.empty_like(q), torch.empty(2, 1, dim, device="cuda")
+    ncz.paged.decode(q, cache, table, lens, o, scale=dim ** -0.5)
+    for h in range(0, group, 5):
+        ncz.paged.decode(q[:, h:h + 1], cache, table, lens, one, scale=dim ** -0.5)
+        # P in 16 bits twice and f32 sums: 2^-9 of o, and 2^-16 of sum p |v| <= max |v| / 16 here
+        limit = 2.0 ** -9 * one[:, 0].abs() + 2.0 ** -16 * float(v.float().abs().max())
+        assert bool(((o[:, h].float() - one[:, 0]).abs() <= limit).all()), h
+    assert ncz.paged.sync_status() == 0
+
+
+def test_decode_wait_that_runs_out(ncz):
+    """A step's scores that are never announced: the kernel stops by itself, the
+    status word says so, and the next call is right again."""
+    pr = wide_problem(4, 20, 1, 64, 16, [300, 400, 500, 600], F16, seed=1)
+    lib = ncz.paged.lib()
+    want, _ = run_decode(ncz, pr, F16)
+    assert lib.ncz_paged_test_set_wait_limit(-1, 2_000_000) == 0  # about 1 ms
+    assert lib.ncz_paged_test_drop_scores(-1, 1) == 0
+    try:
+        run_decode(ncz, pr, F16)
+        with pytest.raises(ncz.FlashError, match="DeviceTimeout"):
+            ncz.paged.sync_status()
+    finally:
+        assert lib.ncz_paged_test_drop_scores(-1, 0) == 0
+        assert lib.ncz_paged_test_set_wait_limit(-1, 0) == 0
+    got, _ = run_decode(ncz, pr, F16)
+    assert ncz.paged.sync_status() == 0 and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 100, 1000])
 def test_decode_window(ncz, window):
     """The pages before a window are given back (-1): nothing of them is read."""
