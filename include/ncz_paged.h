@@ -132,8 +132,9 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * Entries outside [0, num_pages) are absent pages (say, given back once a
  * window has passed them): their keys are left out.  A row without keys gives
  * o = 0 and lse = -infinity.  Nothing in an absent page or behind len affects
- * the result.  Scores, softmax and sums are f32; P is kept in two 16-bit parts
- * (three for bf16 K/V with f32 o).
+ * the result.  Scores, softmax and sums are f32; P goes to the tensor
+ * cores in 16-bit parts: two, but three for bf16 K/V with f32 o and one for
+ * e4m3 K/V with bf16 o.
  *
  * q is f16 or bf16 (the cache's type; either for e4m3); o is f32, f16 or bf16;
  * lse may be NULL, else f32 [batch][q_heads].  q and o may have any strides

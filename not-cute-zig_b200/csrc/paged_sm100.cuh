@@ -390,7 +390,10 @@ struct Decode {
     static constexpr int kSlices = kWarps / kShare;
     static constexpr int kTile = kKeys * kSlices;      // keys per CTA and step
     static constexpr int kStage = kKeys * kRow * 2;    // bytes per slice
-    static constexpr int kCtas = NT == 1 ? 3 : 2;      // CTAs per SM
+    // CTAs per SM: as many as registers allow without spills (128, 168 or 255 a thread).  64 requests
+    // of 4096 keys, 8 K/V heads, f16: head_dim 16 43.2 -> 40.2 us with four instead of three; 16
+    // query heads each, head_dim 32 62.6 -> 55.8 us with three instead of two.
+    static constexpr int kCtas = NT == 1 ? (kRow <= 32 ? 4 : 3) : (D <= 32 && kShare == 1 ? 3 : 2);
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024) / kSlices / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
     static constexpr int kSmem = kSlices * kStages * kStage;
@@ -969,41 +972,44 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
             }
             // P^T fragments in 16-bit parts: each takes the rounded value and leaves the rest to the next.
             uint32_t b[KS][NT][kBf16 ? 3 : 2][2];
-            auto next_part = [&](int ks, int nt, int i) {
+            auto next_part = [&](int ks, int nt, int i, bool more) {
                 float(&x)[4] = s[ks][nt];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t w = pack16<kBf16>(x[2 * h], x[2 * h + 1]);
-                    const float2 back = unpack16<kBf16>(w);
-                    x[2 * h] -= back.x;
-                    x[2 * h + 1] -= back.y;
+                    if (more) {
+                        const float2 back = unpack16<kBf16>(w);
+                        x[2 * h] -= back.x;
+                        x[2 * h + 1] -= back.y;
+                    }
                     b[ks][nt][i][h] = transpose8x8(w);
                 }
             };
+            const bool two = !k8 || p.p_parts > 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    next_part(ks, nt, 0);
-                    next_part(ks, nt, 1);
+                    next_part(ks, nt, 0, two);
+                    if (two) next_part(ks, nt, 1, kBf16 && p.p_parts > 2);
                     if constexpr (kBf16) {
-                        if (p.p_parts > 2) next_part(ks, nt, 2);
+                        if (p.p_parts > 2) next_part(ks, nt, 2, false);
                     }
                 }
-            // The products of a step are summed apart, small parts first, and then added: the
+            // The products of a step are summed apart and then added: the
             // matrix unit's own additions cut off below 2^-24 of the sum, always downwards in
             // magnitude, which over a whole row would leave 1e-6 of it.
             auto block = [&](int ks, int nt, float (&x)[4], bool fresh_sum, uint32_t a0, uint32_t a1, uint32_t a2,
                              uint32_t a3) {
                 const auto &w = b[ks][nt];
                 if (fresh_sum)
-                    mma16816_new<kBf16>(x, a0, a1, a2, a3, w[1][0], w[1][1]);
+                    mma16816_new<kBf16>(x, a0, a1, a2, a3, w[0][0], w[0][1]);
                 else
-                    mma16816<kBf16>(x, a0, a1, a2, a3, w[1][0], w[1][1]);
+                    mma16816<kBf16>(x, a0, a1, a2, a3, w[0][0], w[0][1]);
+                if (two) mma16816<kBf16>(x, a0, a1, a2, a3, w[1][0], w[1][1]);
                 if constexpr (kBf16) {
                     if (p.p_parts > 2) mma16816<kBf16>(x, a0, a1, a2, a3, w[2][0], w[2][1]);
                 }
-                mma16816<kBf16>(x, a0, a1, a2, a3, w[0][0], w[0][1]);
             };
             // Groups without a key are left out: their V rows are not there.
             uint32_t groups = 0;

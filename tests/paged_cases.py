@@ -60,7 +60,7 @@ def plan_oracle(held, added, free_pages, free_count, table, page, capacity):
 
 # ---------------------------------------------------------------- decode
 
-def decode_oracle(q, k_pages, v_pages, table, lens, scale, window=0, k_scale=None, v_scale=None):
+def decode_oracle(q, k_pages, v_pages, table, lens, scale, window=0, k_scale=None, v_scale=None, p_step=2.0 ** -17):
     """(o, lse, tol_o, tol_lse) in float64 from CPU tensors.  The tolerances bound
     a kernel that keeps scores, softmax and sums in f32:
 
@@ -69,7 +69,8 @@ def decode_oracle(q, k_pages, v_pages, table, lens, scale, window=0, k_scale=Non
     order and with truncation), then scaled, offset and put through a
     base-2 exponential (2^-22): ds = (D 2^-23 a + 2^-21 |s|) + 2^-22;
     sums over n keys: at most 2 n / 16 + 64 additions in a chain, each off by 2^-23;
-    P in two bf16 parts (16 bits): 2^-17.
+    P in two bf16 parts (16 bits): 2^-17; `p_step`, where P is given fewer (one f16 part for
+    e4m3 K/V with bf16 o: each weight is off by at most 2^-11 of it, so o by 2^-11 of sum p |v| / l).
     An o is a ratio of two such sums: twice that, of sum p |v| / l."""
     batch, heads, dim = q.shape
     kv = k_pages.shape[2]
@@ -102,7 +103,7 @@ def decode_oracle(q, k_pages, v_pages, table, lens, scale, window=0, k_scale=Non
             magnitude = float((k.abs() @ x.abs() * abs(scale)).max())
             ds = dim * 2.0 ** -23 * magnitude + 2.0 ** -21 * float(s.abs().max()) + 2.0 ** -22
             sums = (2 * len(keys) / 16 + 64) * 2.0 ** -23
-            tol_o[b, h] = 2 * (ds + sums + 2.0 ** -17) * (p @ v.abs())
+            tol_o[b, h] = (2 * (ds + sums) + max(p_step, 2.0 ** -16)) * (p @ v.abs())
             tol_lse[b, h] = ds + sums + 2.0 ** -22 * abs(float(lse[b, h]))
     return o, lse, tol_o, tol_lse
 
