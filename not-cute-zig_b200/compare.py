@@ -15,6 +15,7 @@ src/main.zig:1042); rel = |a - b| / max(|b|, 1e-3).
     python not-cute-zig_b200/compare.py --shape 8,1024,64,1 --gpus 2 --jsonl out.jsonl
     python not-cute-zig_b200/compare.py --shape 4,1000,32,1 --row-stride 40 --in-dtype bf16 --o-dtype f16 --seed 7
     python not-cute-zig_b200/compare.py --mma        # GEMM + epilogue (compareMma, src/main.zig:953-975)
+    python not-cute-zig_b200/compare.py --paged      # decode over the paged cache (no reference counterpart)
     python not-cute-zig_b200/compare.py --join ours.jsonl sdpa.jsonl cuda.jsonl   # joined table
 
 --join reads JSONL records of several harnesses (this one, the reference's
@@ -249,6 +250,59 @@ def compare_mma(ncz, batches: int, k_iters: int, epilogue: int) -> dict:
                       label="mma_gemm_sm100a")
 
 
+def compare_paged(ncz, batch: int, q_heads: int, kv_heads: int, dim: int, keys: int, dtype: str = "f16",
+                  page: int = 16, seed: int = 1) -> dict:
+    """One decode record: `batch` requests of `keys` cached keys in pages of `page`
+    rows in random order, written by paged.append, read by paged.decode (q and O in
+    f16 for an f16 cache, bf16 else; an e4m3 cache with scales of 1/24), checked
+    against plain fp32 attention in torch over the same rows."""
+    import torch
+
+    bench = importlib.import_module("not-cute-zig_b200.benchmark")
+    given = torch.float16 if dtype == "f16" else torch.bfloat16
+    held = {"f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}[dtype]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    per = -(-keys // page)
+    pools = [torch.zeros(batch * per, page, kv_heads, dim, device="cuda", dtype=given).to(held) for _ in range(2)]
+    scale = torch.full((kv_heads,), 1.0 / 24.0, device="cuda") if dtype == "e4m3" else None
+    cache = ncz.paged.Cache(*pools, k_scale=scale, v_scale=scale)
+    table = torch.randperm(batch * per, generator=g, device="cuda").int().view(batch, per)
+    lens = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    key = torch.arange(keys, device="cuda")
+    slots = (table.long()[:, key // page] * page + key % page).view(-1)
+    k, v = (torch.randn(batch * keys, kv_heads, dim, generator=g, device="cuda").to(given) for _ in range(2))
+    ncz.paged.append(k, v, slots, cache)
+    q = torch.randn(batch, q_heads, dim, generator=g, device="cuda").to(given)
+    o = torch.empty_like(q)
+    workspace = ncz.paged.decode_workspace(cache, q_heads)
+    stream = torch.cuda.current_stream()
+    launch = lambda: ncz.paged.decode(q, cache, table, lens, o, scale=dim ** -0.5, workspace=workspace,  # noqa: E731
+                                      stream=stream)
+    el = 1 if dtype == "e4m3" else 2
+    bytes_ = ncz.paged.decode_bytes(batch * keys, batch, q_heads, kv_heads, dim, el)
+    flops = ncz.paged.decode_flops(batch * keys, q_heads, dim)
+    res = bench.run_kernel(launch, warmup_iters=5, iters=20, bytes_processed=bytes_, flops_processed=flops,
+                           stream=stream)
+    ncz.paged.sync_status()
+    max_abs = 0.0
+    for b in range(batch):
+        rows = [x.float()[table[b].long()].reshape(-1, kv_heads, dim)[:keys].transpose(0, 1) for x in pools]
+        if scale is not None:
+            rows = [x * scale[:, None, None] for x in rows]
+        qb = q[b].float().view(kv_heads, q_heads // kv_heads, dim)
+        p = torch.softmax(torch.matmul(qb, rows[0].transpose(1, 2)) * dim ** -0.5, dim=-1)
+        max_abs = max(max_abs, float((o[b].float() - torch.matmul(p, rows[1]).view(q_heads, dim)).abs().max()))
+    peak = measured_hbm()
+    shape = f"batch={batch},q_heads={q_heads},kv_heads={kv_heads},head={dim},keys={keys},page={page},cache={dtype}"
+    return res.record("paged_decode", "not_cute_zig_b200", shape, max_abs <= 0.02, bytes_, flops, max_abs,
+                      pct_hbm_measured=(res.throughput_gbps / peak) if peak else None, host_cores=bench.host_cores(),
+                      label="paged_decode_sm100a")
+
+
+# batch, query heads, K/V heads, head_dim, keys, cache type
+PAGED_SHAPES = [(1, 32, 8, 128, 1000, "bf16"), (64, 16, 16, 64, 2048, "f16"), (64, 32, 8, 128, 4096, "bf16"),
+                (8, 32, 1, 128, 32768, "bf16"), (64, 64, 8, 128, 4096, "e4m3")]
 MMA_SHAPES = [(1, 1, 0), (1 << 21, 1, 1), (1 << 20, 4, 2), (1 << 18, 16, 3)]
 OURS = "not_cute_zig_b200"
 
@@ -312,6 +366,10 @@ def main(argv=None) -> int:
                     help="the GEMM + epilogue records instead: compareMma's 16x8x16 and batched throughput shapes")
     ap.add_argument("--mma-shape", action="append", default=[],
                     help="batches,k_iters,epilogue (repeatable; implies --mma)")
+    ap.add_argument("--paged", action="store_true",
+                    help="records of decode over the paged key-value cache instead")
+    ap.add_argument("--paged-shape", action="append", default=[],
+                    help="batch,q_heads,kv_heads,head,keys,cache type (repeatable; implies --paged)")
     ap.add_argument("--join", nargs="+", default=None, metavar="JSONL",
                     help="print the joined table of these record files (no GPU work)")
     args = ap.parse_args(argv)
@@ -323,6 +381,12 @@ def main(argv=None) -> int:
     if args.mma or args.mma_shape:
         shapes = [tuple(int(x) for x in spec.split(",")) for spec in args.mma_shape] or MMA_SHAPES
         records = [compare_mma(ncz, nb, k, e) for nb, k, e in shapes]
+        bench.emit(records, args.jsonl)
+        return 0 if all(r["correct"] for r in records) else 1
+    if args.paged or args.paged_shape:
+        specs = [spec.split(",") for spec in args.paged_shape]
+        paged_shapes = [(*(int(x) for x in spec[:5]), spec[5]) for spec in specs] or PAGED_SHAPES
+        records = [compare_paged(ncz, *shape) for shape in paged_shapes]
         bench.emit(records, args.jsonl)
         return 0 if all(r["correct"] for r in records) else 1
     shapes = REFERENCE_SHAPES

@@ -1,6 +1,10 @@
 """The paged-cache C ABI on the CPU: refusals (before any launch), grids,
 kernels and workspace through the fake driver table, and the wrapper's checks."""
 import ctypes
+import importlib
+import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -255,3 +259,50 @@ def test_wrapper_refuses_host_tensors(ncz):
     ints = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ncz.FlashError, match="CUDA"):
         ncz.paged.plan(ints, ints, ints, ints[:1], ints.view(2, 2), ints, torch.zeros(4, dtype=torch.int64), page_size=16)
+
+
+@pytest.mark.parametrize("compiler,lang", [("gcc", ["-std=c99"]), ("g++", ["-std=c++17", "-x", "c++"])])
+def test_header_from_c_and_cpp(ncz, tmp_path, compiler, lang):
+    """include/ncz_paged.h as C99 and C++17 without warnings, refusals before any
+    device call (tests/c_abi/paged_consumer.c)."""
+    cc = shutil.which(compiler)
+    if cc is None:
+        pytest.skip(f"no {compiler}")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    libdir = os.path.dirname(ncz.flash.LIB_PATH)
+    exe = tmp_path / "paged_consumer"
+    build = subprocess.run([cc] + lang + ["-Wall", "-Wextra", "-Werror", "-pedantic", "-I", os.path.join(root, "include"),
+                                          os.path.join(root, "tests", "c_abi", "paged_consumer.c"), "-x", "none", "-L",
+                                          libdir, "-lncz_flash", f"-Wl,-rpath,{libdir}", "-o", str(exe)],
+                           capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr
+    ran = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert ran.returncode == 0 and "paged consumer: ok" in ran.stdout, ran.stderr
+
+
+def test_struct_sizes_match_the_header(ncz, tmp_path):
+    """The ctypes mirrors have the sizes and last offsets that the C compiler gives the header's structs."""
+    cc = shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no gcc")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    fields = [("ncz_paged_cache", "dtype"), ("ncz_paged_plan_desc", "stream"), ("ncz_paged_append_desc", "stream"),
+              ("ncz_paged_decode_desc", "stream"), ("ncz_paged_decode_desc", "workspace")]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "ncz_paged.h"\nint main(void) {\n' + "".join(
+        f'    printf("%zu %zu\\n", sizeof({s}), offsetof({s}, {f}));\n' for s, f in fields) + "    return 0;\n}\n")
+    exe = tmp_path / "sizes"
+    subprocess.run([cc, "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = [tuple(int(x) for x in line.split()) for line in
+           subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines()]
+    pg = ncz.paged
+    mirrors = [pg._Cache, pg._Plan, pg._Append, pg._Decode, pg._Decode]
+    assert got == [(ctypes.sizeof(m), getattr(m, f).offset) for m, (_, f) in zip(mirrors, fields)]
+
+
+def test_compare_takes_paged_shapes(ncz, monkeypatch):
+    compare = importlib.import_module("not-cute-zig_b200.compare")
+    seen = []
+    monkeypatch.setattr(compare, "compare_paged", lambda n, *a: seen.append(a) or {"correct": True})
+    assert compare.main(["--paged-shape", "2,8,4,64,100,f16"]) == 0 and seen == [(2, 8, 4, 64, 100, "f16")]
+    assert compare.main(["--paged"]) == 0 and seen[1:] == compare.PAGED_SHAPES

@@ -732,3 +732,12 @@ def test_generate_after_the_forward(ncz):
     used = sum(-(-(m + steps) // page) for m in prompts)
     assert count.tolist() == [pages - used]
     assert ncz.sync_status() == 0
+
+
+def test_compare_paged_record(ncz):
+    import importlib
+
+    compare = importlib.import_module("not-cute-zig_b200.compare")
+    for cache in ("f16", "bf16", "e4m3"):
+        rec = compare.compare_paged(ncz, 3, 8, 2, 64, 333, cache)
+        assert rec["correct"] and rec["kernel"] == "paged_decode", rec
