@@ -75,7 +75,8 @@ int ncz_paged_validate(const ncz_paged_cache *cache);
  * got them): its table row and length stay, its slots are -1, and it takes no
  * page.  No other entry of block_table is touched.  A held page whose table
  * entry is negative gives slot -1.  positions, starts and status may be NULL.
- * Apart from the two pairs named, no output may overlap another array. */
+ * Apart from the two pairs named, no output may overlap another array (lengths
+ * that do are refused).  Arrays are aligned to their elements. */
 typedef struct ncz_paged_plan_desc {
     const int32_t *held;
     const int32_t *added;

@@ -189,7 +189,8 @@ int check_cache(const ncz_paged_cache *c) {
         if (!rows_apart(d, {{strides[i], counts[0]}, {strides[i + 1], counts[1]}, {strides[i + 2], counts[2]}}))
             return NCZ_ERROR_INVALID_VALUE;
     }
-    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return NCZ_ERROR_MISALIGNED;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+        return NCZ_ERROR_MISALIGNED;
     for (int i = 0; i < 6; ++i)
         if (counts[i % 3] > 1 && strides[i] * el % 16 != 0) return NCZ_ERROR_MISALIGNED;
     return NCZ_SUCCESS;
@@ -281,6 +282,19 @@ int ncz_paged_plan(const ncz_paged_plan_desc *desc) {
     if (d.table_width * d.page_size > kMaxInt) return NCZ_ERROR_OVERFLOW;  // positions are 32-bit
     if (d.table_stride > kMaxStride / 2) return NCZ_ERROR_OVERFLOW;
     if (d.requests > 1 && d.table_stride < d.table_width) return NCZ_ERROR_INVALID_VALUE;
+    for (const void *x : {static_cast<const void *>(d.held), static_cast<const void *>(d.added),
+                          static_cast<const void *>(d.free_pages), static_cast<const void *>(d.free_count),
+                          static_cast<const void *>(d.block_table), static_cast<const void *>(d.seq_lens),
+                          static_cast<const void *>(d.positions), static_cast<const void *>(d.starts),
+                          static_cast<const void *>(d.left), static_cast<const void *>(d.status)})
+        if (!aligned(x, 4)) return NCZ_ERROR_MISALIGNED;
+    if (!aligned(d.slots, 8)) return NCZ_ERROR_MISALIGNED;
+    // seq_lens is `held` or apart from it, and apart from `added`.
+    auto overlap = [&](const int32_t *a) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(d.seq_lens);
+        return x < y + 4 * d.requests && y < x + 4 * d.requests;
+    };
+    if (d.requests > 0 && ((d.held != d.seq_lens && overlap(d.held)) || overlap(d.added))) return NCZ_ERROR_INVALID_VALUE;
     nczp::PlanParams p{};
     p.held = d.held;
     p.added = d.added;
@@ -320,7 +334,7 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
     if (c.dtype != NCZ_DTYPE_E4M3 && c.dtype != d.in_dtype) return NCZ_ERROR_INVALID_VALUE;
     if (d.tokens == 0) return NCZ_SUCCESS;
     if (d.k == nullptr || d.v == nullptr || d.slots == nullptr || d.tokens > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
-    if (!aligned(d.k, 2) || !aligned(d.v, 2)) return NCZ_ERROR_MISALIGNED;
+    if (!aligned(d.k, 2) || !aligned(d.v, 2) || !aligned(d.slots, 8)) return NCZ_ERROR_MISALIGNED;
     for (const size_t s : {d.k_token_stride, d.k_head_stride, d.v_token_stride, d.v_head_stride})
         if (s > kMaxStride / 4) return NCZ_ERROR_OVERFLOW;
     const long long el = element_size(c.dtype);
@@ -400,7 +414,9 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     if (!rows_apart(c.head_dim, {{d.o_batch_stride, d.batch}, {d.o_head_stride, d.q_heads}}))
         return NCZ_ERROR_INVALID_VALUE;
     const size_t o_size = static_cast<size_t>(element_size(d.o_dtype));
-    if (!aligned(d.q, 2) || !aligned(d.o, o_size)) return NCZ_ERROR_MISALIGNED;
+    if (!aligned(d.q, 2) || !aligned(d.o, o_size) || !aligned(d.lse, 4) || !aligned(d.block_table, 4) ||
+        !aligned(d.seq_lens, 4))
+        return NCZ_ERROR_MISALIGNED;
     const size_t group = d.q_heads / c.kv_heads;
     nczp::DecodeParams p{};
     p.q = static_cast<const char *>(d.q);

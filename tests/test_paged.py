@@ -102,6 +102,7 @@ def test_cache_layouts_accepted(ncz):
     ({"o_batch_stride": 0}, "InvalidValue"), ({"table_width": 1 << 30, "table_stride": 1 << 30}, "Overflow"),
     ({"q": BASE + 1}, "Misaligned"), ({"o": BASE + 1}, "Misaligned"), ({"workspace": BASE + 8}, "Misaligned"),
     ({"workspace": None}, "OutOfMemory"), ({"workspace_bytes": 1000}, "OutOfMemory"),
+    ({"lse": BASE + 2}, "Misaligned"), ({"seq_lens": BASE + 2}, "Misaligned"), ({"block_table": BASE + 1}, "Misaligned"),
     ({"q_head_stride": 1 << 41}, "Overflow"), ({"device": 64}, "InvalidDevice"),
 ])
 def test_decode_refusals(ncz, fake, over, want):
@@ -120,7 +121,7 @@ def test_decode_accepts_transposed_and_broadcast_rows(ncz, fake):
 @pytest.mark.parametrize("over,want", [
     ({"k": None}, "InvalidValue"), ({"v": None}, "InvalidValue"), ({"slots": None}, "InvalidValue"),
     ({"in_dtype": BF16}, "InvalidValue"), ({"in_dtype": F32}, "InvalidValue"), ({"k": BASE + 1}, "Misaligned"),
-    ({"v_token_stride": 1 << 41}, "Overflow"), ({"tokens": 1 << 31}, "InvalidValue"),
+    ({"slots": BASE + 4}, "Misaligned"), ({"v_token_stride": 1 << 41}, "Overflow"), ({"tokens": 1 << 31}, "InvalidValue"),
 ])
 def test_append_refusals(ncz, fake, over, want):
     assert run(ncz, "ncz_paged_append", cache(ncz), append_desc(ncz, **over)) == want
@@ -133,10 +134,22 @@ def test_append_refusals(ncz, fake, over, want):
     ({"free_count": None}, "InvalidValue"), ({"left": None}, "InvalidValue"), ({"page_size": 0}, "InvalidValue"),
     ({"table_stride": 31}, "InvalidValue"), ({"slot_capacity": 1 << 31}, "InvalidValue"),
     ({"table_width": 1 << 28, "table_stride": 1 << 28}, "Overflow"),
+    ({"seq_lens": BASE + 8}, "InvalidValue"), ({"seq_lens": BASE + 0x10_0000}, "InvalidValue"),  # over held, added
+    ({"held": BASE + 2}, "Misaligned"), ({"slots": BASE + 4}, "Misaligned"), ({"status": BASE + 3}, "Misaligned"),
 ])
 def test_plan_refusals(ncz, fake, over, want):
     assert run(ncz, "ncz_paged_plan", plan_desc(ncz, **over)) == want
     assert fake.launches == []
+
+
+def test_plan_in_place_runs_one_cluster(ncz, fake):
+    """Lengths or the free count in place: another cluster might not have read them."""
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, capacity=100000)) == "Success"
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, capacity=100000, seq_lens=BASE)) == "Success"
+    d = plan_desc(ncz, capacity=100000)
+    d.left = d.free_count
+    assert run(ncz, "ncz_paged_plan", d) == "Success"
+    assert [x.grid for x in fake.launches] == [128, 8, 8]
 
 
 def test_plan_without_optional_outputs(ncz, fake):
