@@ -238,7 +238,11 @@ Choice choose(const ncz_paged_cache &c, size_t group, int o_dtype, size_t batch,
     if (!has_wide(c, group) || o_dtype == NCZ_DTYPE_F32) return narrow;
     const Choice wide = wide_choice(c, group);
     const size_t each = (keys + nczp::kWideTile - 1) / nczp::kWideTile, blocks = (group + wide.rows - 1) / wide.rows;
-    return each >= 4 && batch * c.kv_heads * blocks * each >= 2 * static_cast<size_t>(sms) ? wide : narrow;
+    const size_t total = batch * c.kv_heads * blocks * each, longest = std::min(each, total / sms + 1);
+    // Tensor memory's sums lose up to 7e-8 of themselves a step (measured over 80000 steps): at most a
+    // seventh of the rounding of o over this many steps of a row in one CTA.
+    const size_t limit = o_dtype == NCZ_DTYPE_F16 ? 1024 : 8192;
+    return each >= 4 && total >= 2 * static_cast<size_t>(sms) && longest <= limit ? wide : narrow;
 }
 
 // CTAs of a launch at most: what is resident at once.

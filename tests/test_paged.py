@@ -191,6 +191,12 @@ def test_decode_kernel_for_many_heads_per_kv_head(ncz, fake):
                   label(128, 32, width=24)):
         assert other.startswith("paged_decode<")
     assert label(128, 32, batch=4, kv=8, width=96).startswith("paged_decode_wide<")
+    # tensor memory's sums are kept short beside the output's rounding: steps of one row in one CTA
+    assert label(64, 32, F16, F16, batch=1000, width=1024 * 8).startswith("paged_decode_wide<")
+    assert label(64, 32, F16, F16, batch=1000, width=1025 * 8).startswith("paged_decode<")
+    assert label(64, 32, F16, F16, batch=10, width=1025 * 8).startswith("paged_decode_wide<")
+    assert label(64, 32, batch=1000, width=1025 * 8).startswith("paged_decode_wide<")
+    assert label(64, 32, batch=1000, width=8193 * 8).startswith("paged_decode<")
 
 
 def test_status_word_and_hooks(ncz, fake):
