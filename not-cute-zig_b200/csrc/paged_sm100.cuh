@@ -374,6 +374,7 @@ struct DecodeParams {
 
 constexpr int kWarps = 4;
 constexpr int kDecodeThreads = kWarps * 32;
+constexpr int kDecodeCluster = 8;  // CTAs of a cluster of paged_decode_few
 
 // One instantiation: head_dim, cache type, and the query heads of an item, 8
 // (one matrix column block, NT = 1), 16 (NT = 2) or 32 (NT = 2, two warps
@@ -402,6 +403,7 @@ struct Decode {
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024) / kSlices / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
     static constexpr int kSmem = kSlices * kStages * kStage;
+    static constexpr int kSmemFew = kSmem + kRows * (D + 2) * 4;
     static constexpr int kMaskWords = (kKeys + 31) / 32;
     static constexpr int kCombStride = D + 4;          // floats; 4 apart: no bank conflicts when warps write
     static constexpr int MT = D / 16;                  // 16-row blocks of O^T
@@ -550,17 +552,20 @@ __device__ __forceinline__ void finish_quad(const DecodeParams &p, int b, int kv
 // rescaled rarely (on the first keys, and where scores grow by 2^(kTop-kLift)).
 constexpr float kLift = 8.0f, kTop = 15.0f;
 
-// One new token per request: S^T = K Q^T, P = exp2(f S - base), O^T += V^T P^T, for the query
-// heads of a K/V head at once.  4 G operations meet 2 values of K and V, so up to G = 8 to 16
-// the memory bounds it: the warps are latency machines, 12 or 16 of them an SM with one stage of
-// 8 KB (16 keys of 128 f16) always on its way, 96 KB an SM.  Keys are the rows of the MMAs
-// (m16n8k16) and heads its 8 columns: half the accumulators and MMAs of heads as padded rows of 16,
-// and a key's row is what a warp copies.  Measured: 64 requests of up to 8192 keys, 32 heads of 8,
-// head_dim 128, bf16: 155 us, 6.6 TB/s; 16 heads of head_dim 64, 403 MB: 70 us, 6.4 TB/s behind
-// 7.5 us of latency (launch, lengths, page ids, first rows, join), which is all of a small call
-// (one request of 1000 keys 8.3 us).
-template <class T>
-__global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const DecodeParams p) {
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+    return x;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr) : "memory");
+    return x;
+}
+
+template <class T, bool kCluster>
+__device__ __forceinline__ void decode_body(const DecodeParams &p) {
     constexpr int D = T::D, NT = T::NT, KS = T::KS, MT = T::MT, S = T::kStages;
     constexpr bool kBf16 = T::kKv == kBF16, k8 = T::kKv == kE4M3;
     extern __shared__ __align__(256) char smem[];
@@ -568,6 +573,9 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
     __shared__ int s_start[3];
     __shared__ uint32_t s_mask[kWarps][S][T::kMaskWords];
     __shared__ float s_ml[kWarps][8][2];
+    // kCluster: this CTA's part of the item, behind the ring.
+    float *const s_item = reinterpret_cast<float *>(smem + T::kSmem);
+    float2 *const s_item_ml = reinterpret_cast<float2 *>(s_item + T::kRows * T::D);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int slice = warp / T::kShare, part = warp % T::kShare;  // slice of keys, part of the query heads
@@ -592,7 +600,17 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
     const int run = p.by_head ? blockIdx.x / p.head_blocks : blockIdx.x;
     long long first, last, per;
     Cursor<T::kTile> at;
-    {
+    if constexpr (kCluster) {
+        // One item a cluster, its tiles in eight runs.
+        const int item = blockIdx.x / kDecodeCluster, rank = blockIdx.x % kDecodeCluster;
+        at.b = item / p.head_blocks;
+        at.hb = item % p.head_blocks;
+        request_keys<T::kTile>(p, at.b, at.lo, at.hi, at.tiles);
+        per = (at.tiles + kDecodeCluster - 1) / kDecodeCluster;
+        first = min(rank * per, static_cast<long long>(at.tiles));
+        last = min(first + per, static_cast<long long>(at.tiles));
+        at.tile = static_cast<int>(first);
+    } else {
         const int chunk = (p.batch + kDecodeThreads - 1) / kDecodeThreads;
         const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
         long long mine = 0;
@@ -1134,7 +1152,10 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                         l += ml[1] * f;
                         x = make_float4(x.x + y.x * f, x.y + y.y * f, x.z + y.z * f, x.w + y.w * f);
                     }
-                    if (whole) {
+                    if constexpr (kCluster) {
+                        *reinterpret_cast<float4 *>(s_item + in_block * D + d) = x;
+                        if (d == 0) s_item_ml[in_block] = make_float2(m, l);
+                    } else if (whole) {
                         finish_quad(p, at.b, kv_head, kv_head * p.group + head, d, x, m, l);
                     } else {
                         const long long to = static_cast<long long>(slot) * T::kRows + in_block;
@@ -1145,7 +1166,8 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
                 __syncthreads();
             }
             // The CTA in which an item begins says how many CTAs hold parts of it.
-            if (tid == 0 && !head_cut) {
+            if constexpr (kCluster) {
+            } else if (tid == 0 && !head_cut) {
                 const long long end = step + (at.tiles - at.tile);  // first tile after the item
                 const int ctas = static_cast<int>((end - 1) / per) - run + 1;
                 if (p.records_by_item)
@@ -1162,6 +1184,62 @@ __global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const D
         stage = stage + 1 == S ? 0 : stage + 1;
         at.advance(p);
     }
+
+    if constexpr (kCluster) {
+        // The item's eight parts, each in its CTA's shared memory, joined by all of them in
+        // the same order: a share of the rows' quads each.
+        if (first >= last && tid < T::kRows) s_item_ml[tid] = make_float2(-INFINITY, 0.0f);
+        cluster_sync_all();
+        const int item = blockIdx.x / kDecodeCluster, rank = blockIdx.x % kDecodeCluster;
+        const int b = item / p.head_blocks, hb = item % p.head_blocks;
+        const int kv_head = hb / p.blocks, head0 = (hb - kv_head * p.blocks) * T::kRows;
+        const int quads = min(T::kRows, p.group - head0) * (D / 4);
+        for (int i = rank * kDecodeThreads + tid; i < quads; i += kDecodeCluster * kDecodeThreads) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            float2 ml[kDecodeCluster];
+            float4 y[kDecodeCluster];
+            float m = -INFINITY, l = 0.0f;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kDecodeCluster; ++k) {
+                ml[k] = cluster_load2(cluster_address(smem_u32(s_item_ml + row), k));
+                y[k] = cluster_load4(cluster_address(smem_u32(s_item + row * D + d), k));
+            }
+#pragma unroll
+            for (int k = 0; k < kDecodeCluster; ++k) m = fmaxf(m, ml[k].x);
+#pragma unroll
+            for (int k = 0; k < kDecodeCluster; ++k) {
+                if (ml[k].y == 0.0f) continue;  // no keys: its O was never written
+                const float w = ex2_approx(ml[k].x - m);
+                l += ml[k].y * w;
+                x = make_float4(x.x + y[k].x * w, x.y + y[k].y * w, x.z + y[k].z * w, x.w + y[k].w * w);
+            }
+            finish_quad(p, b, kv_head, kv_head * p.group + head0 + row, d, x, m, l);
+        }
+        cluster_sync_all();  // no CTA leaves while others read its shared memory
+    }
+}
+
+// One new token per request: S^T = K Q^T, P = exp2(f S - base), O^T += V^T P^T, for the query
+// heads of a K/V head at once.  4 G operations meet 2 values of K and V, so up to G = 8 to 16
+// the memory bounds it: the warps are latency machines, 12 or 16 of them an SM with one stage of
+// 8 KB (16 keys of 128 f16) always on its way, 96 KB an SM.  Keys are the rows of the MMAs
+// (m16n8k16) and heads its 8 columns: half the accumulators and MMAs of heads as padded rows of 16,
+// and a key's row is what a warp copies.  Measured: 64 requests of up to 8192 keys, 32 heads of 8,
+// head_dim 128, bf16: 155 us, 6.6 TB/s; 16 heads of head_dim 64, 403 MB: 70 us, 6.4 TB/s behind
+// 7.5 us of latency (launch, lengths, page ids, first rows, join).
+template <class T>
+__global__ void __launch_bounds__(kDecodeThreads, T::kCtas) paged_decode(const DecodeParams p) {
+    decode_body<T, false>(p);
+}
+
+// The same for a few short rows: a cluster of eight CTAs per request and head block, which needs
+// neither the other requests' lengths, nor a workspace, nor paged_join.  All latency: one request
+// of 1000 keys, 8 K/V heads, head_dim 128, bf16: 6.9 us instead of 8.4.
+template <class T>
+__global__ void __cluster_dims__(kDecodeCluster, 1, 1) __launch_bounds__(kDecodeThreads, T::kCtas)
+    paged_decode_few(const DecodeParams p) {
+    decode_body<T, true>(p);
 }
 
 constexpr int kJoinThreads = 256;

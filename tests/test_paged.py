@@ -115,7 +115,7 @@ def test_decode_accepts_transposed_and_broadcast_rows(ncz, fake):
     d = decode_desc(ncz, o_head_stride=4 * 64, o_batch_stride=64, q_head_stride=0)
     assert run(ncz, "ncz_paged_decode", cache(ncz), d) == "Success"
     assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=0, q=None)) == "Success"
-    assert len(fake.launches) == 2
+    assert len(fake.launches) == 1
 
 
 @pytest.mark.parametrize("over,want", [
@@ -167,9 +167,31 @@ def test_decode_kernels_by_type_and_group(ncz, fake):
                 continue
             for group, rows in ((1, 1), (8, 1), (9, 2), (16, 2), (17, 4), (40, 4)):
                 fake.launches.clear()
-                d = decode_desc(ncz, q_heads=2 * group, dim=dim, q_dtype=BF16 if dtype == BF16 else F16)
+                d = decode_desc(ncz, q_heads=2 * group, dim=dim, q_dtype=BF16 if dtype == BF16 else F16, batch=100,
+                                o_dtype=F32)
                 assert run(ncz, "ncz_paged_decode", cache(ncz, kv=2, dim=dim, dtype=dtype), d) == "Success"
                 assert labels(ncz, fake.launches) == [f"paged_decode<{dim},{name},{rows}>", f"paged_join<{dim}>"]
+
+
+def test_decode_kernel_for_few_short_rows(ncz, fake):
+    """A cluster of eight CTAs a row where rows are few and short, no join; else the even shares."""
+    def first(kv, group, batch, keys, dim=128, dtype=BF16, **kw):
+        fake.launches.clear()
+        d = decode_desc(ncz, q_heads=kv * group, dim=dim, q_dtype=F16 if dtype == F16 else BF16, batch=batch,
+                        width=keys // 16, **kw)
+        assert run(ncz, "ncz_paged_decode", cache(ncz, kv=kv, dim=dim, dtype=dtype), d) == "Success"
+        return labels(ncz, fake.launches)
+
+    assert first(8, 4, 1, 1024) == ["paged_decode_few<128,bf16,1>"] and fake.launches[0].grid == 64
+    assert first(8, 12, 1, 1024) == ["paged_decode_few<128,bf16,2>"]
+    assert first(8, 4, 4, 1024) == ["paged_decode_few<128,bf16,1>"] and fake.launches[0].grid == 256
+    assert first(8, 8, 1, 1024, dtype=E4M3) == ["paged_decode_few<128,e4m3,1>"]
+    assert first(1, 1, 1, 1024, 16, F16) == ["paged_decode_few<16,f16,1>"]
+    assert first(8, 4, 1, 16384, window=1000) == ["paged_decode_few<128,bf16,1>"]
+    assert first(8, 4, 1, 4096) == ["paged_decode<128,bf16,1>", "paged_join<128>"]  # too long
+    assert first(8, 4, 5, 1024)[0] == "paged_decode<128,bf16,1>"                     # too many
+    assert first(8, 20, 1, 1024)[0] == "paged_decode<128,bf16,4>"                    # two warps a slice of keys
+    assert first(8, 4, 1, 64) == ["paged_decode<128,bf16,1>"]                        # one tile
 
 
 def test_decode_kernel_for_many_heads_per_kv_head(ncz, fake):
@@ -223,8 +245,8 @@ def test_decode_grid_and_join(ncz, fake):
     assert run(ncz, "ncz_paged_decode", cache(ncz, kv=300), decode_desc(ncz, batch=100, q_heads=300)) == "Success"
     assert fake.launches[0].grid >= grid
     fake.launches.clear()
-    # few rows: join blocks for each of the 8 rows
-    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=1, q_heads=32)) == "Success"
+    # few long rows: join blocks for each of the 8 rows
+    assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=1, q_heads=32, width=512)) == "Success"
     assert fake.launches[1].grid % 8 == 0
     # a window bounds the keys too
     fake.launches.clear()
@@ -252,8 +274,8 @@ def test_launches_go_to_the_named_device_and_count(ncz, fake):
     assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, device=5)) == "Success"
     assert run(ncz, "ncz_paged_append", cache(ncz), append_desc(ncz, device=2)) == "Success"
     assert run(ncz, "ncz_paged_plan", plan_desc(ncz, device=7)) == "Success"
-    assert [x.device for x in fake.launches] == [5, 5, 2, 7] and fake.current() == 0
-    assert ncz.flash.launch_count() - before == 4
+    assert [x.device for x in fake.launches] == [5, 2, 7] and fake.current() == 0
+    assert ncz.flash.launch_count() - before == 3
 
 
 def test_failures_reach_the_caller(ncz, fake):

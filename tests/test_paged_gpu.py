@@ -256,6 +256,9 @@ def test_decode_short_lengths(ncz, dim, dtype, group):
     pr = P.decode_problem(len(LENS), 2 * group, 2, dim, 16, LENS, dtype, seed=dim + group)
     check_decode(ncz, pr, F32)
     check_decode(ncz, pr, dtype)
+    # a table wide enough that rows might be long: even shares over the CTAs instead of clusters
+    pr = P.decode_problem(len(LENS), 2 * group, 2, dim, 16, LENS, dtype, seed=dim + group, width=1500)
+    check_decode(ncz, pr, F32)
 
 
 @pytest.mark.parametrize("dim", [32, 64, 128])
@@ -266,6 +269,8 @@ def test_decode_e4m3(ncz, dim, dtype, group):
     ks, vs = torch.tensor([0.05, 0.031]), torch.tensor([0.02, 1.3])
     check_decode(ncz, pr, F32, k_scale=ks, v_scale=vs)
     check_decode(ncz, pr, dtype, k_scale=ks)
+    pr = P.decode_problem(len(LENS), 2 * group, 2, dim, 8, LENS, dtype, cache_dtype=E4M3, seed=dim + group, width=3000)
+    check_decode(ncz, pr, dtype, k_scale=ks, v_scale=vs)
 
 
 @pytest.mark.parametrize("page", [1, 2, 3, 7, 16, 30, 64, 257])
