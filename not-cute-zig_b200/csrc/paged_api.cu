@@ -523,6 +523,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         p.by_head = choose_by_head(static_cast<size_t>(p.head_blocks), grid);
         if (p.by_head) grid -= grid % static_cast<unsigned>(p.head_blocks);
         p.records_by_item = items <= grid;
+        p.ctas = static_cast<int>(grid);
         char *ws = static_cast<char *>(d.workspace);
         p.records = reinterpret_cast<int4 *>(ws);
         p.part_o = reinterpret_cast<float *>(ws + records_bytes(ctas));

@@ -196,7 +196,7 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
                 refused += s_outcome[c].y;
             }
         }
-        // Slots and positions of this round's tokens.
+        // Slots and positions of the tokens.
         const int *const free_top = p.free_pages + (free_count - 1 - asked);  // read only where a page is left
         const long long room = min(round_tokens, max(0LL, p.slot_capacity - tokens));
         for (long long t = all; t < room; t += stride) {
@@ -369,6 +369,7 @@ struct DecodeParams {
     FastDiv page;
     float scale_log2;
     int records_by_item;
+    int ctas;  // of this launch
     int q_bf16, o_dtype, q_vec, o_vec, p_parts;
 };
 
@@ -1257,9 +1258,15 @@ __global__ void __launch_bounds__(kJoinThreads)
     __shared__ float2 s_ml[kJoinThreads / 32][32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 rec = p.records[blockIdx.x / per_record];
-    const int n = rec.z;
+    const int n = rec.z, next_cta = p.by_head ? p.head_blocks : 1;
     if (n <= 1) return;
-    const int tid = threadIdx.x, lane = tid & 31, next_cta = p.by_head ? p.head_blocks : 1;
+    // A decode kernel that stopped at its wait limit leaves records unwritten: what the workspace
+    // held instead is followed only where it names parts and rows of this launch.
+    if (static_cast<uint32_t>(rec.x) >= static_cast<uint32_t>(p.batch) ||
+        static_cast<uint32_t>(rec.y) >= static_cast<uint32_t>(p.head_blocks) || rec.w < 0 ||
+        rec.w + static_cast<long long>(n - 1) * next_cta >= p.ctas)
+        return;
+    const int tid = threadIdx.x, lane = tid & 31;
     const int sub = tid / quads, subs = kJoinThreads / quads;
     const int quad = (blockIdx.x % per_record) * quads + tid % quads;
     const int row = quad / (D / 4), d = quad % (D / 4) * 4;

@@ -394,6 +394,38 @@ def test_decode_wait_that_runs_out(ncz):
     assert ncz.paged.sync_status() == 0 and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("fill", [0x7F, 0xFF, 0x01, None])
+@pytest.mark.parametrize("lens", [[300, 400, 500, 600], [9000]])
+def test_decode_wait_that_runs_out_on_any_workspace(ncz, lens, fill):
+    """A launch that stops early leaves records of shared rows unwritten: whatever
+    the workspace held there, nothing outside o and lse is touched."""
+    pr = wide_problem(len(lens), 20, 2, 64, 16, lens, F16, seed=3)
+    dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+    cache = ncz.paged.Cache(dev["k"], dev["v"])
+    lib = ncz.paged.lib()
+    workspace = ncz.paged.decode_workspace(cache, 40)
+    if fill is None:
+        workspace.random_(0, 256, generator=torch.Generator(device="cuda").manual_seed(5))
+    else:
+        workspace.fill_(fill)
+    n = pr["q"].numel()
+    around = torch.full((n + 8192,), 3.0, dtype=F16, device="cuda")
+    o = around[4096:4096 + n].view(pr["q"].shape)
+    assert lib.ncz_paged_test_set_wait_limit(-1, 2_000_000) == 0  # about 1 ms
+    assert lib.ncz_paged_test_drop_scores(-1, 1) == 0
+    try:
+        ncz.paged.decode(dev["q"], cache, dev["table"], dev["lens"], o, scale=pr["scale"], workspace=workspace)
+        with pytest.raises(ncz.FlashError, match="DeviceTimeout"):
+            ncz.paged.sync_status()
+    finally:
+        assert lib.ncz_paged_test_drop_scores(-1, 0) == 0
+        assert lib.ncz_paged_test_set_wait_limit(-1, 0) == 0
+    assert bool((around[:4096] == 3).all()) and bool((around[4096 + n:] == 3).all())
+    got, _ = run_decode(ncz, pr, F16, workspace=workspace)
+    want, _ = run_decode(ncz, pr, F16)
+    assert ncz.paged.sync_status() == 0 and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 100, 1000])
 def test_decode_window(ncz, window):
     """The pages before a window are given back (-1): nothing of them is read."""
