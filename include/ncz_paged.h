@@ -89,7 +89,7 @@ typedef struct ncz_paged_plan_desc {
     int32_t *starts;
     int32_t *left;
     int32_t *status;
-    size_t requests;
+    size_t requests; /* at most 2^24 */
     size_t table_width;
     size_t table_stride;  /* elements between rows of block_table */
     size_t free_capacity; /* elements of free_pages; *free_count is clamped to it */
@@ -153,7 +153,7 @@ typedef struct ncz_paged_decode_desc {
     float *lse;
     const int32_t *block_table;
     const int32_t *seq_lens;
-    size_t batch;
+    size_t batch; /* at most 2^24 */
     size_t q_heads;
     size_t table_width;
     size_t table_stride;                  /* elements between rows of block_table */

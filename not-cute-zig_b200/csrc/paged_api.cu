@@ -18,6 +18,7 @@ using ncz::map_cuda_error;
 
 constexpr int kMaxDevices = 64;
 constexpr size_t kMaxInt = 0x7FFFFFFF;
+constexpr size_t kMaxRequests = size_t(1) << 24;
 constexpr size_t kMaxStride = size_t(1) << 40;  // elements; offsets then stay far inside 64 bits
 
 constexpr size_t kPlanClusters = 16, kSlotsPerCluster = 4096;
@@ -313,7 +314,7 @@ int ncz_paged_plan(const ncz_paged_plan_desc *desc) {
     if (d.free_capacity > 0 && d.free_pages == nullptr) return NCZ_ERROR_INVALID_VALUE;
     if (d.slot_capacity > 0 && d.slots == nullptr) return NCZ_ERROR_INVALID_VALUE;
     if (d.page_size == 0 || d.page_size > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
-    if (d.requests > kMaxInt || d.free_capacity > kMaxInt || d.slot_capacity > kMaxInt || d.table_width > kMaxInt)
+    if (d.requests > kMaxRequests || d.free_capacity > kMaxInt || d.slot_capacity > kMaxInt || d.table_width > kMaxInt)
         return NCZ_ERROR_INVALID_VALUE;
     if (d.table_width * d.page_size > kMaxInt) return NCZ_ERROR_OVERFLOW;  // positions are 32-bit
     if (d.table_stride > kMaxStride / 2) return NCZ_ERROR_OVERFLOW;
@@ -442,7 +443,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     if (d.batch == 0) return NCZ_SUCCESS;
     if (d.q == nullptr || d.o == nullptr || d.seq_lens == nullptr || (d.block_table == nullptr && d.table_width > 0))
         return NCZ_ERROR_INVALID_VALUE;
-    if (d.batch > (size_t(1) << 24) || d.table_width > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
+    if (d.batch > kMaxRequests || d.table_width > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
     if (d.table_width * c.page_size > kMaxInt) return NCZ_ERROR_OVERFLOW;
     for (const size_t s : {d.q_batch_stride, d.q_head_stride, d.o_batch_stride, d.o_head_stride, d.table_stride})
         if (s > kMaxStride / 4) return NCZ_ERROR_OVERFLOW;

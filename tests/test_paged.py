@@ -152,6 +152,17 @@ def test_plan_in_place_runs_one_cluster(ncz, fake):
     assert [x.grid for x in fake.launches] == [128, 8, 8]
 
 
+def test_at_most_2_to_the_24_requests(ncz, fake):
+    """The kernels count requests, rounded up to whole rounds, in 32 bits."""
+    wide = {"seq_lens": BASE + (1 << 36), "added": BASE + (1 << 40)}
+    assert run(ncz, "ncz_paged_plan", plan_desc(ncz, requests=1 << 24, **wide)) == "Success"
+    assert len(fake.launches) == 1
+    for n in ((1 << 24) + 1, (1 << 31) - 1):
+        assert run(ncz, "ncz_paged_plan", plan_desc(ncz, requests=n, **wide)) == "InvalidValue"
+        assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, batch=n)) == "InvalidValue"
+    assert len(fake.launches) == 1
+
+
 def test_plan_without_optional_outputs(ncz, fake):
     assert run(ncz, "ncz_paged_plan", plan_desc(ncz, positions=None, starts=None, status=None)) == "Success"
     assert run(ncz, "ncz_paged_plan", plan_desc(ncz, requests=0, held=None, added=None, seq_lens=None,
