@@ -104,10 +104,11 @@ int ncz_paged_plan(const ncz_paged_plan_desc *desc);
 /* Writes rows k[t][h][..] and v[t][h][..] of `tokens` new tokens to the slots
  * slots[t]; a slot below 0 or past the cache is skipped.  f16 and bf16 caches
  * take rows of their own type, unchanged.  An e4m3 cache takes f16 or bf16 rows
- * and holds x / scale[h] rounded to nearest even, values past 448 as 448 (NaN
+ * and holds the f32 quotient x / scale[h] rounded to nearest even, values past 448 as 448 (NaN
  * stays NaN).  k and v may have any strides (rows of head_dim elements).  No
  * slot may be given twice in one call: its row would be that of either token,
- * or parts of both. */
+ * or parts of both.  k and v lie outside the cache, and K and V of the cache are
+ * apart (decode takes a cache that is both at once). */
 typedef struct ncz_paged_append_desc {
     const void *k;
     const void *v;
@@ -139,7 +140,8 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  *
  * q is f16 or bf16 (the cache's type; either for e4m3); o is f32, f16 or bf16;
  * lse may be NULL, else f32 [batch][q_heads].  q and o may have any strides
- * that keep the rows of o apart.
+ * that keep the rows of o apart.  o, lse and workspace overlap nothing else; o in
+ * place of q is refused.
  *
  * The keys of one request and head are split over CTAs that each leave a
  * partial result in `workspace`, joined by a second kernel.  The workspace is
@@ -180,8 +182,8 @@ int ncz_paged_sync_status(int device);
 /* Test hooks (failure detection without a GPU fault), device -1 = current.
  * ncz_paged_test_set_wait_limit: bound of every in-kernel wait in SM cycles (0
  * restores the default, about 2 s).  ncz_paged_test_drop_scores: while enabled,
- * the first CTA of a launch for 17 or more query heads per K/V head never
- * announces its first scores, so a wait runs out. */
+ * the first CTA of a launch of the tcgen05 kernel (many query heads per K/V head)
+ * never announces its first scores, so a wait runs out. */
 int ncz_paged_test_set_wait_limit(int device, uint64_t cycles);
 int ncz_paged_test_drop_scores(int device, int enable);
 

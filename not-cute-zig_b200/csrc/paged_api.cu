@@ -371,6 +371,7 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
     if (c.dtype != NCZ_DTYPE_E4M3 && c.dtype != d.in_dtype) return NCZ_ERROR_INVALID_VALUE;
     if (d.tokens == 0) return NCZ_SUCCESS;
     if (d.k == nullptr || d.v == nullptr || d.slots == nullptr || d.tokens > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
+    if (c.k == c.v) return NCZ_ERROR_INVALID_VALUE;  // each slot would take both rows
     if (!aligned(d.k, 2) || !aligned(d.v, 2) || !aligned(d.slots, 8)) return NCZ_ERROR_MISALIGNED;
     for (const size_t s : {d.k_token_stride, d.k_head_stride, d.v_token_stride, d.v_head_stride})
         if (s > kMaxStride / 4) return NCZ_ERROR_OVERFLOW;
@@ -443,6 +444,8 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     if (d.batch == 0) return NCZ_SUCCESS;
     if (d.q == nullptr || d.o == nullptr || d.seq_lens == nullptr || (d.block_table == nullptr && d.table_width > 0))
         return NCZ_ERROR_INVALID_VALUE;
+    // q is read while o and lse are written.
+    if (d.o == d.q || d.lse == d.q || d.lse == d.o) return NCZ_ERROR_INVALID_VALUE;
     if (d.batch > kMaxRequests || d.table_width > kMaxInt) return NCZ_ERROR_INVALID_VALUE;
     if (d.table_width * c.page_size > kMaxInt) return NCZ_ERROR_OVERFLOW;
     for (const size_t s : {d.q_batch_stride, d.q_head_stride, d.o_batch_stride, d.o_head_stride, d.table_stride})

@@ -203,7 +203,7 @@ def append(k, v, slots, cache: Cache, *, stream=None) -> None:
     whose last is 1) to the cache's slots[t] (int64; -1, or any slot outside the
     cache, is skipped; no slot twice).  A float8_e4m3fn cache takes float16 or
     bfloat16 rows and holds x / scale, rounded and saturated; the others take rows
-    of their own type."""
+    of their own type.  k and v lie outside the cache, whose K and V are apart."""
     torch = _torch
     device = cache.device
     kinds = _KINDS
@@ -240,7 +240,7 @@ def decode(q, cache: Cache, block_table, seq_lens, o, *, scale: float, window: i
     """ncz_paged_decode: o[b, h] = softmax(scale * q[b, h] . K) V over the keys of
     request b, query heads h sharing K/V head h // (q_heads // kv_heads).
 
-    q, o: [batch, q_heads, head_dim], any strides whose last is 1; q float16 or
+    q, o: [batch, q_heads, head_dim], any strides whose last is 1, apart; q float16 or
     bfloat16 (the cache's type; either for a float8_e4m3fn cache), o also
     float32.  block_table: int32 [batch, width], seq_lens: int32 [batch].
     window > 0: only the last `window` keys.  Entries that are no page of the

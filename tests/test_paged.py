@@ -110,6 +110,15 @@ def test_decode_refusals(ncz, fake, over, want):
     assert fake.launches == []
 
 
+def test_outputs_over_inputs_are_refused(ncz, fake):
+    for over in ({"o": BASE}, {"lse": BASE}, {"lse": BASE + 0x100_0000}):
+        assert run(ncz, "ncz_paged_decode", cache(ncz), decode_desc(ncz, **over)) == "InvalidValue"
+    one = cache(ncz, v=BASE)  # K and V in one: for decode only
+    assert run(ncz, "ncz_paged_append", one, append_desc(ncz)) == "InvalidValue"
+    assert fake.launches == []
+    assert run(ncz, "ncz_paged_decode", one, decode_desc(ncz)) == "Success"
+
+
 def test_decode_accepts_transposed_and_broadcast_rows(ncz, fake):
     # o as [q_heads][batch][dim]; one q row for every head
     d = decode_desc(ncz, o_head_stride=4 * 64, o_batch_stride=64, q_head_stride=0)
