@@ -638,6 +638,48 @@ def test_calls_on_another_stream(ncz):
     assert torch.equal(got, want)
 
 
+def test_calls_at_once_on_several_streams(ncz):
+    """Every form of decode (clusters for few rows, even shares with a join, tcgen05),
+    plan and append side by side, eager, each with its own workspace."""
+    problems = [P.decode_problem(2, 8, 2, 128, 16, [900, 31], BF16, seed=1),
+                P.decode_problem(3, 8, 8, 64, 16, [9000, 1, 2500], BF16, seed=2),
+                wide_problem(3, 32, 1, 128, 16, [5000, 0, 7000], BF16, seed=3),
+                wide_problem(2, 20, 2, 64, 16, [6000, 100], BF16, seed=4)]
+    wants = [run_decode(ncz, pr, BF16)[0] for pr in problems]
+    runs = []
+    for pr in problems:
+        dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+        cache = ncz.paged.Cache(dev["k"], dev["v"])
+        runs.append((torch.cuda.Stream(), dev, cache, ncz.paged.decode_workspace(cache, pr["q"].shape[1]),
+                     [torch.zeros(pr["q"].shape, dtype=BF16, device="cuda") for _ in range(8)]))
+    held, added = i32(4 * (np.arange(500) % 9)), i32(np.arange(500) % 5)  # whole pages held: all slots differ
+    free = i32(np.arange(3000)[::-1].copy())
+    plans = [(torch.cuda.Stream(), torch.full((500, 16), 9, dtype=torch.int32, device="cuda"), i32([3000]),
+              torch.zeros(500, dtype=torch.int32, device="cuda"),
+              torch.zeros(1200, dtype=torch.int64, device="cuda")) for _ in range(2)]
+    rows = torch.randn(1200, 2, 64, dtype=BF16, device="cuda")
+    pools = [[torch.zeros(3000, 4, 2, 64, dtype=BF16, device="cuda") for _ in range(2)] for _ in plans]
+    targets = [ncz.paged.Cache(*pool) for pool in pools]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for (stream, dev, cache, workspace, outs), pr in zip(runs, problems):
+            ncz.paged.decode(dev["q"], cache, dev["table"], dev["lens"], outs[i], scale=pr["scale"],
+                             workspace=workspace, stream=stream)
+        for (stream, table, count, lens, slots), target in zip(plans, targets):
+            if i == 0:
+                ncz.paged.plan(held, added, free, count, table, lens, slots, page_size=4, stream=stream)
+            ncz.paged.append(rows, rows, slots, target, stream=stream)
+    torch.cuda.synchronize()
+    assert ncz.paged.sync_status() == 0
+    for (_, _, _, _, outs), want in zip(runs, wants):
+        assert all(torch.equal(o.cpu(), want) for o in outs)
+    slots = plans[0][4]
+    assert int((slots >= 0).sum()) == int(added.sum()) and torch.equal(slots, plans[1][4])
+    for pool in pools:
+        for x in pool:
+            assert torch.equal(x.view(-1, 2, 64)[slots[slots >= 0]], rows[:int(added.sum())])
+
+
 def test_two_graphs_replayed_side_by_side(ncz):
     """Graphs captured without a workspace of their own hold one each."""
     problems = [P.decode_problem(1, 8, 1, 128, 16, [n], BF16, seed=n) for n in (9000, 7001)]
