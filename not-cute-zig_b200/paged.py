@@ -102,21 +102,24 @@ def _fail(what: str):
     raise flash.FlashError(5, what)
 
 
-def _vector(t, dtype, device, what: str, need: int = 0) -> int:
-    """Address of a contiguous CUDA vector of the given type on `device`."""
-    if t.dtype != dtype or t.device != device:
-        _fail(f"{what} must be a {dtype} tensor on {device}")
+# Devices are compared by their index (get_device(), -1 on the host) and types by
+# identity: half of what Device objects and == cost a call, 10 us with the launch.
+
+def _vector(t, dtype, index: int, what: str, need: int = 0) -> int:
+    """Address of a contiguous CUDA vector of the given type on device `index`."""
+    if t.dtype is not dtype or t.get_device() != index:
+        _fail(f"{what} must be a {dtype} tensor on cuda:{index}")
     if t.dim() != 1 or not t.is_contiguous():
         _fail(f"{what} must be a contiguous vector")
-    if t.numel() < need:
+    if need and t.numel() < need:
         _fail(f"{what} holds {t.numel()} elements, needs {need}")
     return t.data_ptr()
 
 
-def _table(t, device, rows: int):
+def _table(t, index: int, rows: int):
     """(address, width, row stride) of a block table."""
-    if t.dtype != _torch.int32 or t.device != device or t.dim() != 2:
-        _fail(f"block_table must be an int32 matrix on {device}")
+    if t.dtype is not _torch.int32 or t.get_device() != index or t.dim() != 2:
+        _fail(f"block_table must be an int32 matrix on cuda:{index}")
     have, width = t.shape
     row, col = t.stride()
     if have < rows:
@@ -126,11 +129,11 @@ def _table(t, device, rows: int):
     return t.data_ptr(), width, row
 
 
-def _stream(stream, device) -> int:
+def _stream(stream, index: int) -> int:
     """Handle of `stream`, by default of the device's current stream (asked for
     without making a Stream object: 0.1 us instead of 2.2 us a call)."""
     if stream is None:
-        return _torch._C._cuda_getCurrentRawStream(device.index)
+        return _torch._C._cuda_getCurrentRawStream(index)
     return flash._stream_handle(stream)
 
 
@@ -153,9 +156,10 @@ class Cache:
         if k.stride(3) != 1 or v.stride(3) != 1:
             _fail("the elements of a row of k and v must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self.index = k.device, k.dtype, k.get_device()
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = k.shape
-        scales = [None if s is None else _vector(s, torch.float32, k.device, "a scale", self.kv_heads)
+        self.row = k.shape[2:]
+        scales = [None if s is None else _vector(s, torch.float32, self.index, "a scale", self.kv_heads)
                   for s in (k_scale, v_scale)]
         self.struct = _Cache(k.data_ptr(), v.data_ptr(), scales[0], scales[1], *k.shape, *k.stride()[:3],
                              *v.stride()[:3], kinds[k.dtype])
@@ -178,7 +182,7 @@ def plan(held, added, free_pages, free_count, block_table, seq_lens, slots, *, p
     refused, tokens past the slots.  A request is refused (slots -1, everything
     else as it was) when its pages do not fit the table's width or the stack."""
     torch = _torch or _load()
-    device, int32 = held.device, torch.int32
+    device, int32 = held.get_device(), torch.int32
     if not held.is_cuda:
         _fail("held must be a CUDA tensor")
     n, capacity = held.numel(), slots.numel()
@@ -194,7 +198,7 @@ def plan(held, added, free_pages, free_count, block_table, seq_lens, slots, *, p
         None if starts is None else _vector(starts, int32, device, "starts", n + 1),
         count if left is None else _vector(left, int32, device, "left", 1),
         None if status is None else _vector(status, int32, device, "status", 4),
-        n, width, row, free_pages.numel(), capacity, page_size, device.index, _stream(stream, device))
+        n, width, row, free_pages.numel(), capacity, page_size, device, _stream(stream, device))
     flash._check(lib().ncz_paged_plan(ctypes.byref(desc)), "paged.plan")
 
 
@@ -204,19 +208,20 @@ def append(k, v, slots, cache: Cache, *, stream=None) -> None:
     cache, is skipped; no slot twice).  A float8_e4m3fn cache takes float16 or
     bfloat16 rows and holds x / scale, rounded and saturated; the others take rows
     of their own type.  k and v lie outside the cache, whose K and V are apart."""
-    torch = _torch
-    device = cache.device
-    kinds = _KINDS
-    if k.dim() != 3 or v.shape != k.shape or k.shape[1] != cache.kv_heads or k.shape[2] != cache.head_dim:
+    index = cache.index
+    shape = k.shape
+    if v.shape != shape or shape[1:] != cache.row:
         _fail(f"k and v must be [tokens, {cache.kv_heads}, {cache.head_dim}]")
-    if k.device != device or v.device != device or k.dtype != v.dtype or k.dtype not in kinds:
-        _fail(f"k and v must be of one type on {device}")
-    ks, vs = k.stride(), v.stride()
-    if ks[2] != 1 or vs[2] != 1:
+    dtype = k.dtype
+    if k.get_device() != index or v.get_device() != index or v.dtype is not dtype or dtype not in _KINDS:
+        _fail(f"k and v must be of one type on {cache.device}")
+    k_tok, k_head, k_one = k.stride()
+    v_tok, v_head, v_one = v.stride()
+    if k_one != 1 or v_one != 1:
         _fail("the elements of a row of k and v must be contiguous")
-    tokens = k.shape[0]
-    desc = _Append(k.data_ptr(), v.data_ptr(), _vector(slots, torch.int64, device, "slots", tokens), tokens, ks[0], ks[1],
-                   vs[0], vs[1], kinds[k.dtype], device.index, _stream(stream, device))
+    tokens = shape[0]
+    desc = _Append(k.data_ptr(), v.data_ptr(), _vector(slots, _torch.int64, index, "slots", tokens), tokens, k_tok, k_head,
+                   v_tok, v_head, _KINDS[dtype], index, _stream(stream, index))
     flash._check(lib().ncz_paged_append(cache.ref, ctypes.byref(desc)), "paged.append")
 
 
@@ -248,31 +253,32 @@ def decode(q, cache: Cache, block_table, seq_lens, o, *, scale: float, window: i
     lse: float32 [batch, q_heads], receives ln of the softmax's sum.  workspace:
     decode_workspace(cache, q_heads); None allocates one for this call (in a
     captured graph: in the graph's own pool)."""
-    device = cache.device
-    kinds = _KINDS
-    if q.dim() != 3 or o.shape != q.shape or q.shape[2] != cache.head_dim:
+    index, kinds = cache.index, _KINDS
+    shape = q.shape
+    if len(shape) != 3 or o.shape != shape or shape[2] != cache.head_dim:
         _fail(f"q and o must be [batch, q_heads, {cache.head_dim}]")
-    if q.device != device or o.device != device or q.dtype not in kinds or o.dtype not in kinds:
-        _fail(f"q and o must be float tensors on {device}")
-    batch, heads, _ = q.shape
-    qs, os_ = q.stride(), o.stride()
-    if qs[2] != 1 or os_[2] != 1:
+    if q.get_device() != index or o.get_device() != index or q.dtype not in kinds or o.dtype not in kinds:
+        _fail(f"q and o must be float tensors on {cache.device}")
+    batch, heads, _ = shape
+    q_batch, q_head, q_one = q.stride()
+    o_batch, o_head, o_one = o.stride()
+    if q_one != 1 or o_one != 1:
         _fail("the elements of a row of q and o must be contiguous")
-    table, width, row = _table(block_table, device, batch)
-    if lse is not None and (lse.shape != q.shape[:2] or lse.device != device or kinds.get(lse.dtype) != 0
+    table, width, row = _table(block_table, index, batch)
+    if lse is not None and (lse.shape != shape[:2] or lse.get_device() != index or lse.dtype is not _torch.float32
                             or not lse.is_contiguous()):
-        _fail(f"lse must be a contiguous float32 tensor [batch, q_heads] on {device}")
+        _fail(f"lse must be a contiguous float32 tensor [batch, q_heads] on {cache.device}")
     if window < 0:
         _fail("window must not be negative")
-    lens = _vector(seq_lens, _torch.int32, device, "seq_lens", batch)
-    handle = _stream(stream, device)
+    lens = _vector(seq_lens, _torch.int32, index, "seq_lens", batch)
+    handle = _stream(stream, index)
     if workspace is None:
         workspace = _call_workspace(cache, heads, stream, handle)
-    elif workspace.device != device or not workspace.is_contiguous():
-        _fail(f"workspace must be a contiguous tensor on {device}")
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        _fail(f"workspace must be a contiguous tensor on {cache.device}")
     desc = _Decode(q.data_ptr(), o.data_ptr(), None if lse is None else lse.data_ptr(), table, lens, batch, heads,
-                   width, row, qs[0], qs[1], os_[0], os_[1], window, scale, kinds[q.dtype], kinds[o.dtype],
-                   workspace.data_ptr(), workspace.numel() * workspace.element_size(), device.index, handle)
+                   width, row, q_batch, q_head, o_batch, o_head, window, scale, kinds[q.dtype], kinds[o.dtype],
+                   workspace.data_ptr(), workspace.nbytes, index, handle)
     flash._check(lib().ncz_paged_decode(cache.ref, ctypes.byref(desc)), "paged.decode")
 
 
