@@ -534,24 +534,25 @@ __device__ __forceinline__ void store_quad(const DecodeParams &p, long long off,
     }
 }
 
-// o = O / L * v_scale and lse = (M + log2 L) ln 2 of one query head; no keys
-// (L = 0): 0 and -infinity.
-__device__ __forceinline__ void finish_quad(const DecodeParams &p, int b, int kv_head, int head, int d, float4 x,
-                                            float m, float l) {
-    const float f = l == 0.0f ? 0.0f : (p.v_scale != nullptr ? __ldg(p.v_scale + kv_head) : 1.0f) / l;
-    store_quad(p, b * p.o_batch + head * p.o_head + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
-    if (d == 0 && p.lse != nullptr) {
-        const long long at = static_cast<long long>(b) * (p.head_blocks / p.blocks) * p.group + head;
-        p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-    }
-}
-
 // The base of the exponentials is kept kLift below the largest score seen
 // when it was set, and raised only when a score passes it by kTop: P then
 // lies in (0, 2^kTop], under the largest f16 value, and keys 2^-kLift further
 // down than with a base at the maximum stay above the smallest f16.  O is
 // rescaled rarely (on the first keys, and where scores grow by 2^(kTop-kLift)).
 constexpr float kLift = 8.0f, kTop = 15.0f;
+
+// o = O / L * v_scale and lse = (M + log2 L) ln 2 of one query head; no keys
+// (L = 0): 0 and -infinity.  M lies kLift below a score and L above 2^kLift: both are
+// moved by that first, or a short row's lse were the small difference of two numbers near 8.
+__device__ __forceinline__ void finish_quad(const DecodeParams &p, int b, int kv_head, int head, int d, float4 x,
+                                            float m, float l) {
+    const float f = l == 0.0f ? 0.0f : (p.v_scale != nullptr ? __ldg(p.v_scale + kv_head) : 1.0f) / l;
+    store_quad(p, b * p.o_batch + head * p.o_head + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+    if (d == 0 && p.lse != nullptr) {
+        const long long at = static_cast<long long>(b) * (p.head_blocks / p.blocks) * p.group + head;
+        p.lse[at] = l == 0.0f ? -INFINITY : ((m + kLift) + log2f(l * 0x1p-8f)) * 0.6931471805599453f;
+    }
+}
 
 __device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
     float4 x;
