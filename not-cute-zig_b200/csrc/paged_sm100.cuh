@@ -96,8 +96,8 @@ __device__ __forceinline__ int last_at_most(const int *start, int n, int bits, i
 // be held, and left be free_count, in place.  Where neither is, several clusters
 // do the same and share the slots and entries (PlanParams; paged_api.cu).
 // Bound by latency (a few KB to 1.2 MB move): 6.3 us for 256 requests of one token, of which
-// 0.9 us is an empty launch; 98304 tokens of 48 prompts 8.4 us with 16 clusters (16.2 with one);
-// 8192 requests of 1 to 7 tokens 13.7 us.
+// 0.9 us is an empty launch; 98304 tokens of 48 prompts 8.6 us with 16 clusters (16.2 with one);
+// 8192 requests of 1 to 7 tokens 13.1 us.
 __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThreads, 1) paged_plan(const PlanParams p) {
     extern __shared__ __align__(16) char plan_smem[];
     // Of a round's requests: new tokens before it (clamped), pages asked for before it (clamped),
