@@ -50,8 +50,15 @@ constexpr int kPlanCluster = 8;
 constexpr int kPlanRound = kPlanThreads * kPlanCluster;  // requests per round: one a thread
 constexpr int kPlanSmem = kPlanRound * sizeof(int4);
 
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -95,9 +102,9 @@ __device__ __forceinline__ int last_at_most(const int *start, int n, int bits, i
 // barriers between reading a round's lengths and writing are what lets seq_lens
 // be held, and left be free_count, in place.  Where neither is, several clusters
 // do the same and share the slots and entries (PlanParams; paged_api.cu).
-// Bound by latency (a few KB to 1.2 MB move): 6.3 us for 256 requests of one token, of which
-// 0.9 us is an empty launch; 98304 tokens of 48 prompts 8.6 us with 16 clusters (16.2 with one);
-// 8192 requests of 1 to 7 tokens 13.1 us.
+// Bound by latency (a few KB to 1.2 MB move): 6.4 us for 256 requests of one token, of which
+// 0.9 us is an empty launch; 98304 tokens of 48 prompts 8.8 us with 16 clusters (16.2 with one);
+// 8192 requests of 1 to 7 tokens 13.2 us.  0.1 us of each is the barrier that the CTAs have started.
 __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThreads, 1) paged_plan(const PlanParams p) {
     extern __shared__ __align__(16) char plan_smem[];
     // Of a round's requests: new tokens before it (clamped), pages asked for before it (clamped),
@@ -107,6 +114,9 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
     __shared__ longlong2 s_totals[kPlanCluster];  // new tokens and pages asked for, by CTA
     __shared__ int2 s_outcome[kPlanCluster];      // pages taken up to there and requests refused, by CTA
     __shared__ int s_taken;
+    // The other CTAs' shared memory may be written only once they have started: all arrive here and
+    // wait in front of the first store, which the loads and the scan of round 0 lie before.
+    cluster_arrive();
     const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool lead = blockIdx.x < kPlanCluster;  // the cluster that writes the lengths and counts
     const int all = blockIdx.x * kPlanThreads + tid, stride = gridDim.x * kPlanThreads;
@@ -158,6 +168,7 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
             }
             a += la;
             b += lb;
+            if (base == 0) cluster_wait();  // the other CTAs have started
             if (tid < kPlanCluster) cluster_store(cluster_address(smem_u32(&s_totals[rank]), tid), wa, wb);
         }
         cluster_sync_all();  // totals; every CTA has read its lengths (and, in round 0, free_count)

@@ -1,0 +1,61 @@
+"""Edges of the paged-cache operators on the GPU that tests/test_paged_gpu.py leaves
+out: calls on a device that is busy, scales and values at the ends of their types, and
+the rounding of P, each against the oracles of tests/paged_cases.py or a bound derived
+beside it."""
+import numpy as np
+import pytest
+
+from tests import paged_cases as P
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("no CUDA device", allow_module_level=True)
+
+F32, F16, BF16, E4M3 = P.F32, P.F16, P.BF16, P.E4M3
+
+
+def i32(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+# ---------------------------------------------------------------- plan
+
+@pytest.mark.parametrize("n", [1, 300, 9000])
+def test_plan_while_other_kernels_hold_the_sms(ncz, n):
+    """Clusters that start when SMs fall free, their CTAs not at the same time: every call's
+    slots, lengths, counts and table are the oracle's."""
+    page, calls = 16, 24
+    rng = np.random.default_rng(n)
+    held = rng.integers(0, 40, n).astype(np.int32)
+    added = rng.integers(0, 5, n).astype(np.int32)
+    width = 4
+    have = -(-held // page)
+    need = -(-(held + added) // page) - have
+    ids = rng.permutation(int(have.sum() + need.sum()) + 5).astype(np.int32)
+    table = np.full((n, width), -1, np.int32)
+    table[np.arange(width)[None, :] < have[:, None]] = ids[:have.sum()]
+    free = ids[have.sum():]
+    capacity = int(added.sum()) + 3
+    want = P.plan_oracle(held, added, free, len(free), table, page, capacity)
+    given = [i32(x) for x in (held, added, free, [len(free)])]
+    outs = []
+    for _ in range(calls):
+        made = lambda k, dt=torch.int32: torch.full((k,), -77, dtype=dt, device="cuda")  # noqa: E731
+        outs.append({"block_table": i32(table), "seq_lens": made(n), "slots": made(capacity, torch.int64),
+                     "positions": made(capacity), "starts": made(n + 1), "left": made(1), "status": made(4)})
+    x = torch.randn(2048, 2048, device="cuda", dtype=BF16)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    busy = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        with torch.cuda.stream(busy):
+            for _ in range(4):
+                x @ x
+        ncz.paged.plan(*given, o["block_table"], o["seq_lens"], o["slots"], page_size=page, positions=o["positions"],
+                       starts=o["starts"], left=o["left"], status=o["status"], stream=streams[i % 4])
+    torch.cuda.synchronize()
+    for o in outs:
+        for name, value in want.items():
+            assert np.array_equal(o[name].cpu().numpy(), value), name
