@@ -183,9 +183,12 @@ int ncz_paged_sync_status(int device);
  * ncz_paged_test_set_wait_limit: bound of every in-kernel wait in SM cycles (0
  * restores the default, about 2 s).  ncz_paged_test_drop_scores: while enabled,
  * the first CTA of a launch of the tcgen05 kernel (many query heads per K/V head)
- * never announces its first scores, so a wait runs out. */
+ * never announces its first scores, so a wait runs out.  ncz_paged_test_leave_merge:
+ * while enabled, one of the four softmax warps of that CTA gives up where its first
+ * item ends, as at a wait that ran out, while the others are about to merge. */
 int ncz_paged_test_set_wait_limit(int device, uint64_t cycles);
 int ncz_paged_test_drop_scores(int device, int enable);
+int ncz_paged_test_leave_merge(int device, int enable);
 
 /* Bytes of workspace for ncz_paged_decode on `device` (-1 = current). */
 int ncz_paged_decode_workspace(const ncz_paged_cache *cache, size_t q_heads, int device, size_t *bytes);

@@ -581,6 +581,13 @@ int ncz_paged_test_drop_scores(int device, int enable) {
     });
 }
 
+int ncz_paged_test_leave_merge(int device, int enable) {
+    const int v = enable != 0;
+    return on_device(device, [&](int) {
+        return map_cuda_error(drv().symbol_write(static_cast<const void *>(&nczp::g_paged_test_leave), &v, sizeof(v)));
+    });
+}
+
 }  // extern "C"
 
 namespace ncz {

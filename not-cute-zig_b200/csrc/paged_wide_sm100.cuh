@@ -33,7 +33,8 @@
 //
 // Every mbarrier wait is bounded.  On expiry the waiter records itself in
 // g_paged_status and raises the CTA's abort flag; the roles leave their loops,
-// copies and MMAs in flight are waited for, tensor memory is freed.
+// copies and MMAs in flight are waited for, tensor memory is freed.  The softmax
+// warps' hardware barriers have no limit of their own: see softmax_together.
 #pragma once
 #include "paged_sm100.cuh"
 
@@ -42,7 +43,8 @@ namespace nczp {
 constexpr unsigned long long kPagedWaitLimit = 4000000000ull;  // SM cycles, about 2 s
 __device__ uint32_t g_paged_status = 0u;
 __device__ unsigned long long g_paged_wait_limit = kPagedWaitLimit;
-__device__ int g_paged_test_drop = 0;  // test hook: the first step's scores are never announced
+__device__ int g_paged_test_drop = 0;   // test hook: the first step's scores are never announced
+__device__ int g_paged_test_leave = 0;  // test hook: a softmax warp gives up where the first item ends
 
 // Where a bounded wait gave up (bits 24.. of the status word).
 enum : uint32_t {
@@ -85,9 +87,13 @@ struct Wide {
 // must be within one phase of it: what belongs to a step has a barrier per score
 // buffer, whose next phase cannot come before the step that waits.
 struct WideBars {
-    uint64_t full[12], empty[12], q_full[2], s_full[2], p_full[2], o_done[2], o_free, merge, drain[2];
+    uint64_t full[12], empty[12], q_full[2], s_full[2], p_full[2], o_done[2], o_free, drain[2];
 };
 
+__device__ __forceinline__ void paged_give_up(volatile uint32_t *abort_flag, uint32_t site) {
+    *abort_flag = 1u;
+    atomicCAS(&g_paged_status, 0u, 0x80000000u | (site << 24) | (blockIdx.x & 0xFFFFFFu));
+}
 __device__ __noinline__ bool paged_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag,
                                              uint32_t site, bool honor_abort) {
     const unsigned long long t0 = ncz::sm_clock();
@@ -96,8 +102,7 @@ __device__ __noinline__ bool paged_wait_slow(uint32_t bar, uint32_t parity, vola
         if ((it & 15u) == 0u) {
             if (honor_abort && *abort_flag) return false;
             if (ncz::sm_clock() - t0 > g_paged_wait_limit) {
-                *abort_flag = 1u;
-                atomicCAS(&g_paged_status, 0u, 0x80000000u | (site << 24) | (blockIdx.x & 0xFFFFFFu));
+                paged_give_up(abort_flag, site);
                 return false;
             }
         }
@@ -149,7 +154,23 @@ __device__ __forceinline__ void umma_ts_lanes(uint32_t d, uint32_t high, uint32_
     }
 }
 
-// Hardware barrier of the four softmax warps.
+// Hardware barriers of the four softmax warps.
+//
+// softmax_together: whether all four come with `ok`.  Each warp calls it once for every
+// item that it ends, or, where one of its waits ran out first, once with false as it leaves,
+// so all four are in the same call; a warp that hears false leaves and calls no barrier
+// again.  Between two calls a warp waits at limited waits only, hence every call ends.
+// softmax_sync: only between a call that said true and the end of that item, where no warp can leave.
+__device__ __forceinline__ bool softmax_together(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n.reg .pred mine, all;\nsetp.ne.b32 mine, %1, 0;\nbar.red.and.pred all, 1, 128, mine;\n"
+        "selp.b32 %0, 1, 0, all;\n}\n"
+        : "=r"(all)
+        : "r"(ok ? 1u : 0u)
+        : "memory");
+    return all != 0;
+}
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <class T>
@@ -182,7 +203,6 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
             ncz::mbar_init(smem_u32(&bars.p_full[i]), 4);
         }
         ncz::mbar_init(smem_u32(&bars.o_free), 4);
-        ncz::mbar_init(smem_u32(&bars.merge), 4);
         ncz::mbar_init(smem_u32(&bars.drain[0]), 1);
         ncz::mbar_init(smem_u32(&bars.drain[1]), 1);
         s_abort = 0;
@@ -420,20 +440,16 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars.q_full[item & 1]));
             };
-            int merges = 0;
-            // The four warps meet (bounded: mbarrier, not a hardware barrier).
-            auto meet = [&]() {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars.merge));
-                return paged_wait(&bars.merge, merges++ & 1, abort_flag, kSiteMerge);
-            };
+            const bool leave = g_paged_test_leave != 0 && blockIdx.x == 0 && warp == 1;
             float base = -INFINITY, sum = 0.0f;
             int item = 0;
-            bool opens = true, head_cut = at.tile != 0, ok = true;
+            bool opens = true, head_cut = at.tile != 0;
+            bool gave_up = false;  // this warp, at a wait; the others hear of it in softmax_together
             load_q(at.b, at.hb, 0);
-            for (int j = 0; j < steps && ok; ++j) {
+            for (int j = 0; j < steps; ++j) {
                 const uint32_t t_s = tmem + t_lane + (j & 1) * 128 + copy * kCols;
-                if (!paged_wait(&bars.s_full[j & 1], (j >> 1) & 1, abort_flag, kSiteScores)) break;
+                gave_up = !paged_wait(&bars.s_full[j & 1], (j >> 1) & 1, abort_flag, kSiteScores);
+                if (gave_up) break;
                 ncz::tc_fence_after();
                 uint32_t x[kCols];
                 if constexpr (kCols == 32) ncz::tmem_ld_x32_wait(t_s, x);
@@ -460,7 +476,8 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                     sum *= down;
                     if (!opens) {
                         // O is rescaled after P V of the step before.
-                        if (!paged_wait(&bars.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, kSiteODone)) break;
+                        gave_up = !paged_wait(&bars.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, kSiteODone);
+                        if (gave_up) break;
                         ncz::tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < D; c += 16) {
@@ -522,7 +539,12 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                             if (d == 0) p.part_ml[part0 + r] = make_float2(top_, l);
                         }
                     };
-                    if (!paged_wait(&bars.o_done[j & 1], (j >> 1) & 1, abort_flag, kSiteODone)) break;
+                    gave_up = !paged_wait(&bars.o_done[j & 1], (j >> 1) & 1, abort_flag, kSiteODone);
+                    if (leave) {
+                        paged_give_up(abort_flag, kSiteMerge);
+                        gave_up = true;
+                    }
+                    if (gave_up) break;
                     ncz::tc_fence_after();
                     if constexpr (kCopies == 1) {
 #pragma unroll
@@ -535,12 +557,9 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                                                             __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3])), base, sum);
                         }
                     } else {
-                        // The copies' states through shared memory, 16 columns at a time.  Once the
-                        // four warps have met, none of them can stop before they are through, so
-                        // hardware barriers will do.
+                        // The copies' states through shared memory, 16 columns at a time.
                         s_ml[tid] = make_float2(base, sum);
-                        ok = meet();
-                        if (!ok) break;
+                        if (!softmax_together(true)) break;
                         // This thread's quads of 16 columns: rows r0 + 32 i, the same ones in every chunk.
                         constexpr int kQuads = T::kQRows / 32;
                         const int r0 = tid / 4, d0 = tid % 4 * 4;
@@ -605,6 +624,7 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                 }
                 at.advance(p);
             }
+            if (kCopies > 1 && gave_up) softmax_together(false);
         }
     }
     ncz::tc_fence_before();

@@ -67,6 +67,7 @@ _SIGNATURES = {
     "ncz_paged_sync_status": (ctypes.c_int, [ctypes.c_int]),
     "ncz_paged_test_set_wait_limit": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint64]),
     "ncz_paged_test_drop_scores": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
+    "ncz_paged_test_leave_merge": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
     "ncz_paged_decode_workspace": (ctypes.c_int, [ctypes.POINTER(_Cache), _SZ, ctypes.c_int, ctypes.POINTER(_SZ)]),
 }
 _bound: Optional[ctypes.CDLL] = None

@@ -31,3 +31,22 @@ def test_cluster_memory_is_touched_after_a_cluster_barrier():
         assert touch and passed and passed.start() < touch.start(), name
         if passed.group(1) == "wait":
             assert re.search(r"\bcluster_arrive\(\)", text[:passed.start()]), name
+
+
+def test_softmax_warps_leave_a_hardware_barrier_together():
+    """bar.sync has no limit, so no softmax warp of paged_decode_wide may stand at one that
+    another has left: they enter the merge by a vote that all four take part in, also those
+    that stopped at a limited wait, and nothing between the vote and the end of the item leaves."""
+    text = body("paged_wide_sm100.cuh", "paged_decode_wide")
+    softmax = text[text.index("const int copy = warp"):]
+    assert "softmax_sync" not in text[:len(text) - len(softmax)]
+    enter = softmax.index("if (!softmax_together(true)) break;")
+    last = softmax.rindex("softmax_sync();")
+    assert enter < softmax.index("softmax_sync();")
+    assert not re.search(r"\bbreak\b|\breturn\b|paged_wait", softmax[enter + len("if (!softmax_together(true)) break;"):last])
+    # every other way out of the loop says so first, and votes once behind it
+    exits = [m.start() for m in re.finditer(r"\bbreak;", softmax)]
+    assert len(exits) == 4
+    for at in exits:
+        assert softmax[:at].endswith(("if (gave_up) ", "if (!softmax_together(true)) "))
+    assert last < exits[-1] or re.search(r"gave_up\) softmax_together\(false\);", softmax[max(last, exits[-1]):])

@@ -59,3 +59,34 @@ def test_plan_while_other_kernels_hold_the_sms(ncz, n):
     for o in outs:
         for name, value in want.items():
             assert np.array_equal(o[name].cpu().numpy(), value), name
+
+
+# ---------------------------------------------------------------- decode, many query heads per K/V head
+
+@pytest.mark.parametrize("dim,group", [(64, 20), (128, 20), (64, 40), (128, 64), (64, 100), (128, 128)])
+@pytest.mark.parametrize("lens", [[300, 400, 500, 600], [9000]])
+def test_decode_stops_when_one_softmax_warp_gives_up_at_the_merge(ncz, dim, group, lens):
+    """One of the four warps that merge an item leaves just before: the others must not wait for
+    it.  The launch ends, the status word says so, and the next call is right again."""
+    pr = P.decode_problem(len(lens), group, 1, dim, 16, lens, F16, width=-(-(148 * 2 * 128) // 16), seed=dim + group)
+    dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+    cache = ncz.paged.Cache(dev["k"], dev["v"])
+    outs = [torch.zeros(pr["q"].shape, dtype=F16, device="cuda") for _ in range(3)]
+    lib = ncz.paged.lib()
+
+    def call(o):
+        ncz.paged.decode(dev["q"], cache, dev["table"], dev["lens"], o, scale=pr["scale"])
+
+    call(outs[0])
+    assert ncz.paged.sync_status() == 0
+    assert lib.ncz_paged_test_set_wait_limit(-1, 2_000_000) == 0  # about 1 ms
+    assert lib.ncz_paged_test_leave_merge(-1, 1) == 0
+    try:
+        call(outs[1])
+        with pytest.raises(ncz.FlashError, match="DeviceTimeout"):
+            ncz.paged.sync_status()
+    finally:
+        assert lib.ncz_paged_test_leave_merge(-1, 0) == 0
+        assert lib.ncz_paged_test_set_wait_limit(-1, 0) == 0
+    call(outs[2])
+    assert ncz.paged.sync_status() == 0 and torch.equal(outs[0], outs[2])
