@@ -148,7 +148,8 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * at least the bytes that ncz_paged_decode_workspace reports for the cache and
  * q_heads, 16-byte aligned, for any batch; it needs no initial contents and
  * keeps none.  Calls that may run at the same time (streams, or captured graphs
- * replayed side by side) each need their own. */
+ * replayed side by side) each need their own; calls on one stream may share one,
+ * whichever host threads make them. */
 typedef struct ncz_paged_decode_desc {
     const void *q;
     void *o;

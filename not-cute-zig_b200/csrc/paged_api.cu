@@ -26,6 +26,13 @@ constexpr size_t kPlanClusters = 16, kSlotsPerCluster = 4096;
 std::mutex g_mu;
 int g_sms[kMaxDevices];
 
+// Held over a decode launch and its join, by stream: another thread's decode on the same stream,
+// which may use the same workspace, must not come between the two.
+std::mutex g_pair_mu[64];
+std::mutex &pair_mutex(int dev, const void *stream) {
+    return g_pair_mu[(reinterpret_cast<uintptr_t>(stream) / 64 * 31 + static_cast<uintptr_t>(dev)) % 64];
+}
+
 // One instantiation: its address, label, shared memory and what of it has been set up.
 struct Kernel {
     const void *fn;
@@ -533,9 +540,11 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
         p.part_o = reinterpret_cast<float *>(ws + records_bytes(ctas));
         p.part_ml = reinterpret_cast<float2 *>(p.part_o + 2 * static_cast<size_t>(ctas) * rows * c.head_dim);
         void *args[1] = {&p};
-        int s = launch(k, grid, k.threads, dev, d.stream, args);
         // Rows of one tile are whole in one CTA: nothing to join.
-        if (s != NCZ_SUCCESS || most == 1) return s;
+        if (most == 1) return launch(k, grid, k.threads, dev, d.stream, args);
+        std::lock_guard<std::mutex> lock(pair_mutex(dev, d.stream));
+        const int s = launch(k, grid, k.threads, dev, d.stream, args);
+        if (s != NCZ_SUCCESS) return s;
         // Quads (four elements) per join block: as few as keep the grid within
         // four blocks an SM, a 128-byte line of a part's row at least.
         const unsigned records = p.records_by_item ? static_cast<unsigned>(items) : grid;
