@@ -499,6 +499,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return kBf16 ? ncz::pack_bf16x2(lo, hi) : ncz::pack_f16x2(lo, hi);
 }
 
+// Two elements of Q times a factor of 0: 0, or NaN where they are not finite.  With them and a factor
+// of 1 a finite score is 0 and a masked one stays -infinity, which 0 times it would not.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t times_zero16(uint32_t w) {
+    constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;  // all of it set: infinity or NaN
+    const uint32_t lo = (w & kExp) == kExp ? 0x7FFFu : 0u, hi = ((w >> 16) & kExp) == kExp ? 0x7FFF0000u : 0u;
+    return lo | hi;
+}
+
 // Keys of request b: [lo, hi), in `tiles` tiles from lo rounded down to 16
 // (one tile at least, so that every request's rows are written).
 template <int kTile>
@@ -888,9 +897,14 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) qf[kk][nt][j] ^= 0x80008000u;
                 }
-                // Not 0: masked scores stay -infinity times it.  1e-35 of any finite score is 0 beside a 1.
                 up *= fabsf(scale);
-                up = up == 0.0f ? 1e-35f : up;
+                if (up == 0.0f) {
+                    up = 1.0f;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) qf[kk][nt][j] = times_zero16<kBf16>(qf[kk][nt][j]);
+                }
                 f[nt][0] = __shfl_sync(~0u, up, (2 * t4) * 4);
                 f[nt][1] = __shfl_sync(~0u, up, (2 * t4 + 1) * 4);
                 base[nt][0] = base[nt][1] = -INFINITY;

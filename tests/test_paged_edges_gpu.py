@@ -90,3 +90,51 @@ def test_decode_stops_when_one_softmax_warp_gives_up_at_the_merge(ncz, dim, grou
         assert lib.ncz_paged_test_set_wait_limit(-1, 0) == 0
     call(outs[2])
     assert ncz.paged.sync_status() == 0 and torch.equal(outs[0], outs[2])
+
+
+# ---------------------------------------------------------------- decode, scales and values at the ends of their types
+
+@pytest.mark.parametrize("dim,group,width,out", [(64, 2, 40, F32), (128, 4, 2400, BF16), (64, 20, 2400, BF16),
+                                                 (128, 40, 2400, BF16), (32, 20, 40, BF16)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-45])
+def test_decode_of_large_bf16_scores_at_scale_zero(ncz, dim, group, width, out, scale):
+    """Scores of 1e36 times 0 are 0: every key weighs the same, o is the mean of V and lse = ln n.
+    (1e-45, the smallest f32, times log2 e stays the smallest f32: scores of 1e-9, below f32's
+    step at a weight of 1.)  Bounds: weights are exact, V's sum of n terms is off by at most
+    n 2^-23 of sum |v|, o by a rounding; log2 of up to 300 by 2^-20 (f32's step at 8), lse by 2^-22 more."""
+    lens = [1, 300, 129, 0, 17]
+    pr = P.decode_problem(5, 2 * group, 2, dim, 16, lens, BF16, seed=dim + group, width=width)
+    pr["q"] *= 1e18
+    pr["k"] = torch.where(torch.isnan(pr["k"]), pr["k"], pr["k"] * 1e17)
+    dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+    o = torch.full(pr["q"].shape, 7.0, dtype=out, device="cuda")
+    lse = torch.full(pr["q"].shape[:2], 7.0, device="cuda")
+    ncz.paged.decode(dev["q"], ncz.paged.Cache(dev["k"], dev["v"]), dev["table"], dev["lens"], o, scale=scale, lse=lse)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert bool((o[b] == 0).all()) and bool((lse[b] == -torch.inf).all())
+            continue
+        rows = torch.cat([pr["v"][int(pr["table"][b, j])] for j in range(-(-n // 16))])[:n].double()
+        mean, size = rows.mean(0), rows.abs().mean(0)
+        want = mean.repeat_interleave(group, 0)
+        limit = ((n + 4) * 2.0 ** -23 * size + P.half_step(out) * (mean.abs() + size * 2.0 ** -12)).repeat_interleave(group, 0)
+        assert bool(((o[b].cpu().double() - want).abs() <= limit).all()), b
+        assert float((lse[b].cpu().double() - np.log(n)).abs().max()) <= 2.0 ** -19, b
+
+
+@pytest.mark.parametrize("dim,group,width", [(64, 2, 40), (64, 20, 2400), (128, 40, 2400)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_decode_scale_zero_keeps_nan_and_infinity(ncz, dim, group, width, dtype):
+    """0 times an infinite or NaN score is NaN, in the rows of that query or key alone."""
+    pr = P.decode_problem(3, 2 * group, 2, dim, 16, [40, 50, 60], dtype, seed=dim, width=width)
+    pr["q"][0, 0, 3] = float("inf")
+    pr["q"][1, 1, 0] = float("nan")
+    pr["k"][int(pr["table"][2, 1]), 5, 1, 7] = float("inf")
+    dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+    o = torch.zeros(pr["q"].shape, dtype=dtype, device="cuda")
+    ncz.paged.decode(dev["q"], ncz.paged.Cache(dev["k"], dev["v"]), dev["table"], dev["lens"], o, scale=0.0)
+    bad = torch.isnan(o).all(-1)
+    want = torch.zeros_like(bad)
+    want[0, 0] = want[1, 1] = True
+    want[2, group:] = True
+    assert torch.equal(torch.isnan(o).any(-1), bad) and torch.equal(bad, want)
