@@ -134,7 +134,9 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * Entries outside [0, num_pages) are absent pages (say, given back once a
  * window has passed them): their keys are left out.  A row without keys gives
  * o = 0 and lse = -infinity.  Nothing in an absent page or behind len affects
- * the result.  Scores, softmax and sums are f32; P goes to the tensor
+ * the result.  Scores, softmax and sums are f32.  bf16 q over an e4m3 cache is held in
+ * f16, times a power of two of its row: elements below 2^-17 of the row's largest one are
+ * off by at most 2^-25 of that, the others are exact.  P goes to the tensor
  * cores in 16-bit parts: two, but three for bf16 K/V with f32 o and one for
  * e4m3 K/V with bf16 o.
  *

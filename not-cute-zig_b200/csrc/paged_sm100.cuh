@@ -840,7 +840,13 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p) {
             fresh = false;
             const int kv_head = p.blocks == 1 ? at.hb : at.hb / p.blocks;
             const int head0 = (at.hb - kv_head * p.blocks) * T::kRows + part * (8 * NT);  // of the group
-            const float scale = p.scale_log2 * (k8 && p.k_scale != nullptr ? __ldg(p.k_scale + kv_head) : 1.0f);
+            // Over an 8-bit cache the factor has three parts whose product fits f32 where two of them may not.
+            const auto scale = [&]() {
+                if constexpr (k8)
+                    return static_cast<double>(p.scale_log2) * (p.k_scale != nullptr ? __ldg(p.k_scale + kv_head) : 1.0f);
+                else
+                    return p.scale_log2;
+            }();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int head = head0 + nt * 8 + g;
@@ -866,7 +872,9 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p) {
                     if (p.q_bf16) {
                         // bf16 spans more than f16: take a power of two out of the row, so
                         // that its largest element lies in [1, 2); what f16 then rounds is below
-                        // 2^-25 of that element.
+                        // 2^-25 of that element.  The power is 2^-126 to 2^126, so that its inverse is a
+                        // normal float too: the largest rows come to [2, 4), and rows of subnormals
+                        // to multiples of 2^-7 below 1, which f16 holds exactly.
                         float top = 0.0f;
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
@@ -877,11 +885,9 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p) {
                             }
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                        const uint32_t e = (__float_as_uint(top) >> 23) & 255u;
-                        // 2^(e-127) and its inverse, both normal floats for 1 <= e <= 253
-                        const bool in = e >= 1 && e <= 253;
-                        up = in ? __uint_as_float(e << 23) : 1.0f;
-                        const float down = in ? __uint_as_float((254u - e) << 23) : 1.0f;
+                        const uint32_t e = min(max((__float_as_uint(top) >> 23) & 255u, 1u), 253u);
+                        up = __uint_as_float(e << 23);
+                        const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
@@ -891,13 +897,13 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p) {
                             }
                     }
                 }
-                if (scale < 0.0f) {
+                if (scale < 0) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) qf[kk][nt][j] ^= 0x80008000u;
                 }
-                up *= fabsf(scale);
+                up = static_cast<float>(up * fabs(scale));
                 if (up == 0.0f) {
                     up = 1.0f;
 #pragma unroll

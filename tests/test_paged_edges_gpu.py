@@ -138,3 +138,30 @@ def test_decode_scale_zero_keeps_nan_and_infinity(ncz, dim, group, width, dtype)
     want[0, 0] = want[1, 1] = True
     want[2, group:] = True
     assert torch.equal(torch.isnan(o).any(-1), bad) and torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("dim,group", [(32, 3), (64, 16), (128, 8)])
+@pytest.mark.parametrize("top", [127, -133])
+def test_decode_bf16_queries_at_the_ends_of_their_range_over_e4m3(ncz, dim, group, top):
+    """Rows of q whose largest element is 1.5 2^127, or the smallest bf16 there is, against an
+    8-bit cache: as the definition says, not infinity or 0.  Scores as in decode_oracle."""
+    lens = [70, 3, 200]
+    pr = P.decode_problem(3, 2 * group, 2, dim, 16, lens, BF16, cache_dtype=E4M3, seed=dim + group, fill=0.0)
+    pr["k"] = (pr["k"].float() / 384).to(E4M3)
+    g = torch.Generator().manual_seed(top + 200)
+    sign = torch.where(torch.rand(pr["q"].shape, generator=g) < 0.5, -1.0, 1.0)
+    if top > 0:
+        q = sign.double() * 1.5 * 2.0 ** 127 * (torch.rand(pr["q"].shape, generator=g) < 0.5)
+    else:
+        q = sign.double() * 2.0 ** -133
+    pr["q"] = q.to(BF16)
+    k_scale = torch.tensor([1.0, 0.5]) if top > 0 else torch.tensor([2.0 ** 60, 2.0 ** 61])
+    pr["scale"] = 2.0 ** -125 if top > 0 else 2.0 ** 75
+    want, want_lse, tol, tol_lse = P.decode_oracle(pr["q"], pr["k"], pr["v"], pr["table"], pr["lens"], pr["scale"],
+                                                   0, k_scale)
+    dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+    o, lse = torch.zeros(pr["q"].shape, device="cuda"), torch.zeros(pr["q"].shape[:2], device="cuda")
+    ncz.paged.decode(dev["q"], ncz.paged.Cache(dev["k"], dev["v"], k_scale=k_scale.cuda()), dev["table"], dev["lens"], o,
+                     scale=pr["scale"], lse=lse)
+    assert bool(((o.cpu().double() - want).abs() <= tol + P.half_step(F32) * want.abs()).all())
+    assert bool(((lse.cpu().double() - want_lse).abs() <= tol_lse).all())
