@@ -138,7 +138,8 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * f16, times a power of two of its row: elements below 2^-17 of the row's largest one are
  * off by at most 2^-25 of that, the others are exact.  P goes to the tensor
  * cores in 16-bit parts: two, but three for bf16 K/V with f32 o and one for
- * e4m3 K/V with bf16 o.
+ * e4m3 K/V with bf16 o.  bf16 parts for bf16 K/V; f16 parts else, in which the weight of
+ * a key is off by up to 2^-33 of the row's largest as well.
  *
  * q is f16 or bf16 (the cache's type; either for e4m3); o is f32, f16 or bf16;
  * lse may be NULL, else f32 [batch][q_heads].  q and o may have any strides

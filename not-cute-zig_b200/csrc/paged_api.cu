@@ -501,8 +501,12 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
     p.q_vec = aligned(d.q, 8) && d.q_batch_stride % 4 == 0 && d.q_head_stride % 4 == 0;
     p.o_vec = aligned(d.o, 4 * o_size) && d.o_batch_stride % 4 == 0 && d.o_head_stride % 4 == 0;
     // 16-bit parts of P: f32 o takes the bits of f32 (3 of bf16, 2 of f16), 16-bit o two parts as
-    // well.  One f16 part (2^-11) is eight times finer than bf16 o (2^-8); for e4m3 K/V, where the
-    // conversions keep the SM busy, that is 3 % of the time (48 requests, 64 query heads of 8: 152 -> 147 us).
+    // well.  One f16 part (2^-11 of a weight) is eight times finer than bf16 o (2^-8); for e4m3 K/V, where
+    // the conversions keep the SM busy, a second one costs 2 % with 8 query heads a K/V head (16 requests of
+    // 8192 keys, 4 K/V heads, head_dim 128: 33.6 and 34.3 us) and 8 % with 32 (69.3 and 74.8).
+    // f16's smallest step is 2^-24 and a row's largest P 2^8 or more, so in f16 parts, however many, a
+    // weight is also off by up to 2^-33 of the row's largest: that is the larger error below 2^-22 of
+    // it with one part, below 2^-11 with two, and weights below 2^-33 are in the sum but not in o.
     p.p_parts = c.dtype == NCZ_DTYPE_BF16 && d.o_dtype == NCZ_DTYPE_F32 ? 3
                 : c.dtype == NCZ_DTYPE_E4M3 && d.o_dtype == NCZ_DTYPE_BF16 ? 1 : 2;
 

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from tests import paged_cases as P
+from tests import paged_edge_cases as E
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +166,60 @@ def test_decode_bf16_queries_at_the_ends_of_their_range_over_e4m3(ncz, dim, grou
                      scale=pr["scale"], lse=lse)
     assert bool(((o.cpu().double() - want).abs() <= tol + P.half_step(F32) * want.abs()).all())
     assert bool(((lse.cpu().double() - want_lse).abs() <= tol_lse).all())
+
+
+# ---------------------------------------------------------------- decode, the rounding of P
+
+KINDS = [(F16, F16, F32), (F16, F16, F16), (BF16, BF16, F32), (BF16, BF16, BF16), (BF16, E4M3, BF16), (BF16, E4M3, F32),
+         (F16, E4M3, F16), (F16, E4M3, F32)]
+
+
+@pytest.mark.parametrize("dim,group,width", [(32, 1, 1), (64, 8, 40), (128, 12, 40), (128, 20, 2400)])
+@pytest.mark.parametrize("q_dtype,dtype", [(F16, F16), (BF16, BF16), (BF16, E4M3), (F16, E4M3)])
+def test_decode_one_weight_in_f32(ncz, dim, group, width, q_dtype, dtype):
+    """f32 o holds a weight to f32's bits: P goes to the tensor cores in as many parts as that takes."""
+    b = E.two_keys(dtype)
+    n, page = len(b), 16
+    k, v = (torch.zeros(n, page, 1, dim) for _ in range(2))
+    k[:, 1, 0, 0] = b
+    v[:, 1] = 1.0
+    q = torch.zeros(n, group, dim, dtype=q_dtype, device="cuda")
+    q[..., 0] = 1.0
+    table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(n)
+    o, lse = torch.zeros(n, group, dim, device="cuda"), torch.zeros(n, group, device="cuda")
+    cache = ncz.paged.Cache(k.to(dtype).cuda(), v.to(dtype).cuda())
+    ncz.paged.decode(q, cache, table, i32([2] * n), o, scale=1.0, lse=lse)
+    w = torch.exp(b.double())[:, None, None]
+    kind, count = E.parts_of(dtype, F32)
+    limit = E.TWO_KEYS_BOUND + E.weight_error(kind, count)[0]
+    assert float(((o.cpu().double() - w / (1 + w)).abs() / (w / (1 + w))).max()) <= limit
+    # ln of the sum: 5.25 2^-22 of it as above, log2 (2^-23) and a rounding of up to 0.7
+    assert float((lse.cpu().double() - torch.log1p(w[..., 0])).abs().max()) <= 7 * 2.0 ** -22
+
+
+@pytest.mark.parametrize("down", [10.3, 21.7, 25.3, 29.6, 33.0, 36.5])
+@pytest.mark.parametrize("n,group,width", [(3000, 2, 0), (700, 20, 2400), (700, 3, 0), (700, 70, 2400)])
+@pytest.mark.parametrize("q_dtype,dtype,out", KINDS)
+def test_decode_sum_of_small_weights(ncz, n, group, width, q_dtype, dtype, out, down):
+    """Thousands of keys far below one: their sum is kept to the rounding of P's parts, which for
+    f16 parts has an absolute term of 2^-33 of the largest weight a key."""
+    dim, page = 64, 16
+    pages = -(-n // page)
+    k, v = torch.zeros(pages, page, 1, dim), torch.ones(pages, page, 1, dim)
+    scale = down * float(np.log(2))
+    k[pages // 2, 3, :, 0] = 1.0
+    v[pages // 2, 3] = 0.0
+    q = torch.zeros(1, group, dim, dtype=q_dtype, device="cuda")
+    q[..., 0] = 1.0
+    table = torch.full((1, max(width, pages)), -1, dtype=torch.int32, device="cuda")
+    table[0, :pages] = torch.arange(pages)
+    o = torch.zeros(1, group, dim, dtype=out, device="cuda")
+    cache = ncz.paged.Cache(k.to(dtype).cuda(), v.to(dtype).cuda())
+    ncz.paged.decode(q, cache, table, i32([n]), o, scale=scale)
+    want, w = E.tail_want(n, -float(np.float32(scale)))
+    kind, count = E.parts_of(dtype, out)
+    limit = E.tail_bound(n, w, want, kind, count)
+    limit += P.half_step(out) * (want + limit) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+    assert float((o.cpu().double() - want).abs().max()) <= limit, (want, limit)
+    assert ncz.paged.sync_status() == 0

@@ -1,7 +1,11 @@
-"""The paged-cache entry points from several host threads, on fake devices."""
+"""The paged-cache entry points from several host threads, on fake devices, and what the
+GPU tests' rounding bounds can tell apart."""
 import ctypes
 import threading
 
+import torch
+
+from tests import paged_edge_cases as E
 from tests.test_paged import BASE, cache, decode_desc, labels
 
 
@@ -34,3 +38,14 @@ def test_decodes_of_two_threads_on_one_stream_keep_their_joins(ncz, fake):
     names = labels(ncz, fake.launches)
     assert [n.split("<")[0] for n in names] == ["paged_decode", "paged_join"] * 2
     assert {x.stream for x in fake.launches} == {stream}
+
+
+def test_the_two_key_rows_tell_the_parts_of_p_apart():
+    """The bound that tests/test_paged_edges_gpu.py holds f32 outputs to is below the error that
+    one part fewer would give, and above that of the parts there are."""
+    for dtype in (E.F16, E.BF16, E.E4M3):
+        kind, count = E.parts_of(dtype, E.F32)
+        p = 256 * torch.exp(E.two_keys(dtype).double())
+        error = lambda n: float(((E.in_parts(p, kind, n) - p).abs() / p).max())  # noqa: E731
+        assert error(count) <= E.weight_error(kind, count)[0] + 2.0 ** -24
+        assert error(count - 1) > 1.5 * E.TWO_KEYS_BOUND
