@@ -262,10 +262,12 @@ Choice wide_choice(const ncz_paged_cache &c, size_t group) {
 // the tcgen05 kernel takes 128 keys a step and starts and ends slower (32 query
 // heads of 8 K/V heads, head_dim 128: one request of 2000 keys, 128 steps in all,
 // 14.4 us with the warp MMAs and 15.0 us with it, of 8000 keys 23.6 and 19.3;
-// 64 requests of 300 keys, 3 steps each, 46.1 and 52.4, of 1000 keys 92.0 and 73.2).
-Choice choose(const ncz_paged_cache &c, size_t group, int o_dtype, size_t batch, size_t keys, int sms) {
+// 64 requests of 300 keys, 3 steps each, 46.1 and 52.4, of 1000 keys 92.0 and 73.2).  So does a scale of
+// 0, which takes a Q of its own (nczp::times_zero16): the registers for that cost the
+// tcgen05 kernel up to 8 % of every other launch.
+Choice choose(const ncz_paged_cache &c, size_t group, int o_dtype, float scale_log2, size_t batch, size_t keys, int sms) {
     const Choice narrow = narrow_choice(c, group);
-    if (!has_wide(c, group) || o_dtype == NCZ_DTYPE_F32) return narrow;
+    if (!has_wide(c, group) || o_dtype == NCZ_DTYPE_F32 || scale_log2 == 0.0f) return narrow;
     const Choice wide = wide_choice(c, group);
     const size_t each = (keys + nczp::kWideTile - 1) / nczp::kWideTile, blocks = (group + wide.rows - 1) / wide.rows;
     const size_t total = batch * c.kv_heads * blocks * each, longest = std::min(each, total / sms + 1);
@@ -515,7 +517,7 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
 
     return on_device(d.device, [&](int dev) {
         const int sms = device_sms(dev);
-        const Choice choice = choose(c, group, d.o_dtype, d.batch, keys, sms);
+        const Choice choice = choose(c, group, d.o_dtype, p.scale_log2, d.batch, keys, sms);
         Kernel &k = *choice.kernel;
         const int rows = choice.rows;
         const size_t blocks = (group + rows - 1) / rows;

@@ -405,8 +405,7 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
             // ---- softmax: query head `row` of the item, keys kCols copy .. of each step.
             const int copy = warp / (4 / kCopies), row = warp % (4 / kCopies) * 32 + lane;
             const uint32_t t_lane = static_cast<uint32_t>(warp * 32) << 16;
-            const bool zero = p.scale_log2 == 0.0f;  // Q is times_zero16 of it then, and the factor 1
-            const float f = zero ? 1.0f : fabsf(p.scale_log2);
+            const float f = fabsf(p.scale_log2);  // not 0 (paged_api.cu:choose): masked scores stay -infinity
             const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
             // Q of an item into tensor memory: this lane's query head.
             auto load_q = [&](int b, int hb, int item) {
@@ -433,7 +432,7 @@ __global__ void __launch_bounds__(T::kThreads, 1) paged_decode_wide(const Decode
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t x[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = zero ? times_zero16<kBf16>(w[c + i]) : w[c + i] ^ flip;
+                    for (int i = 0; i < 16; ++i) x[i] = w[c + i] ^ flip;
                     ncz::tmem_st_x16(t_q + t_lane + (item & 1) * (D / 2) + c, x);
                 }
                 ncz::tmem_wait_st();

@@ -49,3 +49,14 @@ def test_the_two_key_rows_tell_the_parts_of_p_apart():
         error = lambda n: float(((E.in_parts(p, kind, n) - p).abs() / p).max())  # noqa: E731
         assert error(count) <= E.weight_error(kind, count)[0] + 2.0 ** -24
         assert error(count - 1) > 1.5 * E.TWO_KEYS_BOUND
+
+
+def test_scale_zero_takes_the_warp_mmas(ncz, fake):
+    """They alone turn Q into 0 times itself."""
+    c = cache(ncz, kv=1)
+    for scale, kernel in ((0.125, "paged_decode_wide"), (-0.125, "paged_decode_wide"), (1e-45, "paged_decode_wide"),
+                          (0.0, "paged_decode"), (-0.0, "paged_decode")):
+        fake.launches.clear()
+        d = decode_desc(ncz, q_heads=32, batch=64, scale=scale)
+        assert ncz.paged.lib().ncz_paged_decode(ctypes.byref(c), ctypes.byref(d)) == 0
+        assert labels(ncz, fake.launches)[0].split("<")[0] == kernel, scale
