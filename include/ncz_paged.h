@@ -40,7 +40,7 @@ typedef struct ncz_paged_cache {
     const float *v_scale;
     size_t num_pages;
     size_t page_size; /* any number of rows >= 1 */
-    size_t kv_heads;
+    size_t kv_heads; /* at most 65536 */
     size_t head_dim; /* 16 (not e4m3), 32, 64 or 128 */
     size_t k_page_stride, k_token_stride, k_head_stride; /* elements */
     size_t v_page_stride, v_token_stride, v_head_stride;
@@ -76,7 +76,11 @@ int ncz_paged_validate(const ncz_paged_cache *cache);
  * page.  No other entry of block_table is touched.  A held page whose table
  * entry is negative gives slot -1.  positions, starts and status may be NULL.
  * Apart from the two pairs named, no output may overlap another array (lengths
- * that do are refused).  Arrays are aligned to their elements. */
+ * that do are refused).  Arrays are aligned to their elements.
+ *
+ * Where seq_lens is `held` or left is free_count, 8 SMs do the work, else up to 128:
+ * the same time for a step of one token each, twice that for long prompts (98304 new
+ * tokens of 48 requests 16.2 and 8.8 us). */
 typedef struct ncz_paged_plan_desc {
     const int32_t *held;
     const int32_t *added;
@@ -146,6 +150,11 @@ int ncz_paged_append(const ncz_paged_cache *cache, const ncz_paged_append_desc *
  * that keep the rows of o apart.  o, lse and workspace overlap nothing else; o in
  * place of q is refused.
  *
+ * The lengths are on the device, so the kernel and the grid are chosen by the longest
+ * row there may be, table_width * page_size keys (or window, if that is less): a table
+ * much wider than its rows costs short rows time (one request of 1000 keys, 8 K/V heads,
+ * head_dim 128: 7.1 us with a table of 1024 keys, 8.8 of 2048, 9.8 of 131072).
+ *
  * The keys of one request and head are split over CTAs that each leave a
  * partial result in `workspace`, joined by a second kernel.  The workspace is
  * at least the bytes that ncz_paged_decode_workspace reports for the cache and
@@ -160,7 +169,7 @@ typedef struct ncz_paged_decode_desc {
     const int32_t *block_table;
     const int32_t *seq_lens;
     size_t batch; /* at most 2^24 */
-    size_t q_heads;
+    size_t q_heads; /* at most 65536, a multiple of the cache's kv_heads */
     size_t table_width;
     size_t table_stride;                  /* elements between rows of block_table */
     size_t q_batch_stride, q_head_stride; /* elements */
@@ -180,7 +189,9 @@ int ncz_paged_decode(const ncz_paged_cache *cache, const ncz_paged_decode_desc *
 /* Synchronises `device` (-1 = current), then reads and clears the bounded-wait
  * status word of its decode kernels: NCZ_SUCCESS, or NCZ_ERROR_DEVICE_TIMEOUT
  * when a wait inside a kernel ran past the wait limit since the last call (that
- * kernel then stopped cleanly; its o and lse are incomplete). */
+ * kernel then stopped cleanly; its o and lse are incomplete).  The forward's and the
+ * GEMM's status words are their own (ncz_flash_sync_status, ncz_mma_sync_status): a
+ * program that checks its steps asks for each kind of kernel it ran. */
 int ncz_paged_sync_status(int device);
 
 /* Test hooks (failure detection without a GPU fault), device -1 = current.

@@ -24,8 +24,8 @@
 //
 // A step's 128 keys are 64 KB of K and V at head_dim 128: 1.4 us at the memory's rate, in
 // which the SM issues 8 + 16 MMAs and the softmax takes about 1000 cycles.  Measured (batch 16,
-// 4 K/V heads, 8192 keys, bf16): 32 query heads each, head_dim 128 58.5 us (4.6 TB/s; the warp
-// MMAs 86.5), 64 heads 67 us (153), head_dim 64 41 us (57); 3 requests of up to 131072 keys with
+// 4 K/V heads, 8192 keys, bf16): 32 query heads each, head_dim 128 59 us (4.5 TB/s; the warp
+// MMAs 86.5), 64 heads 67 us (153), head_dim 64 43 us (57); 3 requests of up to 131072 keys with
 // one K/V head 41 us, of which 17 us stream at the memory's rate and the rest is latency.
 //
 // S is double buffered: Q K^T of step j + 1 runs while the softmax works on

@@ -393,7 +393,9 @@ def launch_multi(descs: Sequence[_Desc]) -> None:
 
 def sync_status(device: Optional[int] = None, stream=None) -> int:
     """Synchronises the stream and raises FlashError(DeviceTimeout) if a
-    bounded in-kernel wait expired since the last call; returns the raw word."""
+    bounded in-kernel wait of the forward expired since the last call; returns the raw
+    word.  The GEMM and the paged cache have words of their own (mma.sync_status,
+    paged.sync_status)."""
     detail = ctypes.c_uint32(0)
     handle = 0 if stream is None else _stream_handle(stream)
     st = lib().ncz_flash_sync_status(-1 if device is None else device, handle, ctypes.byref(detail))

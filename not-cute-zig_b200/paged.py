@@ -10,7 +10,9 @@ The reference has no cache and no decoding step (its attention takes whole K/V
 slices, src/flash.zig:31-70).  Tensors are torch CUDA tensors of one device; calls
 run asynchronously on `stream` (default: that device's current stream), whatever
 the current device is, and can be captured into CUDA graphs.  Errors raise
-FlashError with the library's status code.
+FlashError with the library's status code.  A bounded wait that ran out inside decode
+is reported by this module's sync_status alone (flash.sync_status and mma.sync_status
+are those of the forward and the GEMM).
 """
 from __future__ import annotations
 
@@ -181,7 +183,11 @@ def plan(held, added, free_pages, free_count, block_table, seq_lens, slots, *, p
     starts: int32 [requests + 1]; left: int32 [1], the stack's new count (default:
     free_count itself); status: int32 [4], new tokens, pages taken, requests
     refused, tokens past the slots.  A request is refused (slots -1, everything
-    else as it was) when its pages do not fit the table's width or the stack."""
+    else as it was) when its pages do not fit the table's width or the stack.
+
+    With seq_lens or left in place (left is, by default) 8 SMs do the work: the same time
+    for a step of one token each, twice the time for long prompts (98304 new tokens 16.2 us
+    instead of 8.8)."""
     torch = _torch or _load()
     device, int32 = held.get_device(), torch.int32
     if not held.is_cuda:
@@ -253,7 +259,9 @@ def decode(q, cache: Cache, block_table, seq_lens, o, *, scale: float, window: i
     cache leave their keys out; a row without keys gives o = 0 and lse = -inf.
     lse: float32 [batch, q_heads], receives ln of the softmax's sum.  workspace:
     decode_workspace(cache, q_heads); None allocates one for this call (in a
-    captured graph: in the graph's own pool)."""
+    captured graph: in the graph's own pool).  The kernel is chosen by the longest row that
+    the table's width (or the window) allows: a table no wider than it has to be is faster
+    for short rows (one request of 1000 keys 7.1 us, with a table of 131072 keys 9.8)."""
     index, kinds = cache.index, _KINDS
     shape = q.shape
     if len(shape) != 3 or o.shape != shape or shape[2] != cache.head_dim:
