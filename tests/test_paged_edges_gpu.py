@@ -223,3 +223,47 @@ def test_decode_sum_of_small_weights(ncz, n, group, width, q_dtype, dtype, out, 
     limit += P.half_step(out) * (want + limit) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
     assert float((o.cpu().double() - want).abs().max()) <= limit, (want, limit)
     assert ncz.paged.sync_status() == 0
+
+
+# ---------------------------------------------------------------- host threads
+
+def test_host_threads_share_a_stream_and_a_workspace(ncz):
+    """Three threads decode on one stream with one workspace, rows that take a join: every call's
+    output is that of the same call alone, bit for bit."""
+    import threading
+
+    problems = [P.decode_problem(n, 8, 2, 128, 16, [2500 + 100 * i for i in range(n)], BF16, seed=n) for n in (2, 3, 5)]
+    stream = torch.cuda.Stream()
+    calls, workspace = [], None
+    for pr in problems:
+        dev = {n: pr[n].cuda() for n in ("q", "k", "v", "table", "lens")}
+        cache = ncz.paged.Cache(dev["k"], dev["v"])
+        workspace = ncz.paged.decode_workspace(cache, 8) if workspace is None else workspace
+        outs = torch.zeros(100, *pr["q"].shape, dtype=BF16, device="cuda")
+        calls.append((dev, cache, pr["scale"], outs))
+    want = []
+    for dev, cache, scale, outs in calls:
+        ncz.paged.decode(dev["q"], cache, dev["table"], dev["lens"], outs[0], scale=scale)
+        want.append(outs[0].clone())
+        outs[0].zero_()
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(3), []
+
+    def work(dev, cache, scale, outs):
+        try:
+            start.wait()
+            for o in outs:
+                ncz.paged.decode(dev["q"], cache, dev["table"], dev["lens"], o, scale=scale, workspace=workspace,
+                                 stream=stream)
+        except Exception as e:  # a thread's exception must fail the test
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert failed == []
+    for (_, _, _, outs), w in zip(calls, want):
+        assert bool((outs == w).all())
