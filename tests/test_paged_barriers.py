@@ -49,4 +49,4 @@ def test_softmax_warps_leave_a_hardware_barrier_together():
     assert len(exits) == 4
     for at in exits:
         assert softmax[:at].endswith(("if (gave_up) ", "if (!softmax_together(true)) "))
-    assert last < exits[-1] or re.search(r"gave_up\) softmax_together\(false\);", softmax[max(last, exits[-1]):])
+    assert re.search(r"if \(kCopies > 1 && gave_up\) softmax_together\(false\);", softmax[max(last, exits[-1]):])
